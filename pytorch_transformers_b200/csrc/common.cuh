@@ -20,6 +20,7 @@ enum {
   PTB_ERR_SIZE = 2,       // a size that the kernel does not take
   PTB_ERR_LAUNCH = 3,     // the launch itself failed (cudaGetLastError)
   PTB_ERR_ALIGN = 4,      // a pointer or a row size that is not aligned as the kernel needs
+  PTB_ERR_PAGES = 5,      // cache pages that cannot be copied as asked
 };
 
 // Activations, by the codes that every entry point with an `act` argument takes. This is the one table:

@@ -7,9 +7,12 @@ calls fail.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import native
@@ -19,7 +22,8 @@ PAGE = 64  # tokens of a cache page (PTB_PAGE in csrc/common.cuh)
 ACTIVATIONS = {"none": 0, "gelu": 1, "gelu_new": 2, "gelu_pytorch_tanh": 2, "relu": 3, "relu2": 4, "silu": 5}   # relu2: relu(x)^2
 NORM_KINDS = {"layernorm": 0, "rmsnorm": 1}
 _ERRORS = {1: "unknown dtype code", 2: "a size that the kernel does not take", 3: "the CUDA launch failed",
-           4: "a pointer or row size is not aligned as the kernel needs"}
+           4: "a pointer or row size is not aligned as the kernel needs",
+           5: "a page out of range, named twice as a target, or source and target at once"}
 
 
 class KernelError(RuntimeError):
@@ -115,12 +119,14 @@ def lib():
                      "ptb_qk_prepare_store", "ptb_route_grouped", "ptb_expert_combine_shared", "ptb_glu_act",
                      "ptb_head_norm_gate_act", "ptb_gla_decay", "ptb_gla_walk", "ptb_gla_chunks", "ptb_gla_max_dim",
                      "ptb_gla_chunk_tokens", "ptb_delta_prepare", "ptb_delta_walk", "ptb_delta_chunks",
-                     "ptb_delta_chunks_supports", "ptb_post_norm", "ptb_token_gate", "ptb_round_rows", "ptb_route_biased", "ptb_attention_tc_sizes", "ptb_attention_tc_supports_sizes", "ptb_attention_tc_extras"):
+                     "ptb_delta_chunks_supports", "ptb_post_norm", "ptb_token_gate", "ptb_round_rows", "ptb_route_biased", "ptb_attention_tc_sizes", "ptb_attention_tc_supports_sizes", "ptb_attention_tc_extras",
+                     "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_q8_splits", "ptb_attention_decode_q8", "ptb_attention_q8"):
             getattr(L, name).restype = ctypes.c_int
         L.ptb_latent_part_floats.restype = ctypes.c_longlong
         L.ptb_rglru_chunks_work_floats.restype = ctypes.c_longlong
         L.ptb_expert_plan_words.restype = ctypes.c_longlong
         L.ptb_mlstm_chunks_scratch_floats.restype = ctypes.c_longlong
+        L.ptb_attention_q8_floats.restype = ctypes.c_longlong
         _configured = True
     return L
 
@@ -1767,3 +1773,230 @@ def round_rows(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         raise KernelError("round_rows takes float32 rows to bfloat16")
     _check(lib().ptb_round_rows(_ptr(x), _ptr(out), ctypes.c_longlong(x.numel()), _stream(x)), "round_rows")
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# A cache in 8 bits: e4m3 codes [pages, kv_heads, PAGE, head_dim] and one exponent [pages, kv_heads] (int8) for each page and
+# K/V head; a value is code * 2^exponent. csrc/q8.cuh says why a power of two.
+Q8 = torch.float8_e4m3fn
+Q8_MAX_HEADS = 128       # query heads a K/V head in attention_decode_q8
+
+
+def q8_supports(head_dim: int) -> bool:
+    return 16 <= head_dim <= 256 and head_dim % 16 == 0
+
+
+def _on_device(t: torch.Tensor):
+    """The device guard of ``t``'s device where it is not the current one (a launch goes to a stream of the current device)."""
+    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Tensor, seq_new: torch.Tensor, seq_past: torch.Tensor,
+               pages: torch.Tensor) -> StepBatchC:
+    """The description of a step for the kernels from int32 tensors on the device (``StepContext`` builds it for the engine):
+    sequence and position of every token, each sequence's first token, tokens of this step and tokens before it, and the page
+    table [sequences, width]. The tensors must outlive the kernels that read them."""
+    for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages):
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise KernelError("step_batch takes contiguous int32 tensors on the device")
+    n = seq_start.numel()
+    if tok_seq.numel() != tok_pos.numel() or seq_new.numel() != n or seq_past.numel() != n or pages.dim() != 2 or pages.shape[0] != n:
+        raise KernelError("step_batch: the arrays' lengths do not fit one another")
+    return StepBatchC(tok_seq.data_ptr(), tok_pos.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), seq_past.data_ptr(),
+                      pages.data_ptr(), pages.shape[1], tok_seq.numel(), n)
+
+
+def _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads: int, head_dim: int, device, what: str) -> None:
+    for pool, exp in ((k_pool, k_exp), (v_pool, v_exp)):
+        if (pool.dtype != Q8 or exp.dtype != torch.int8 or pool.dim() != 4 or pool.shape[1:] != (kv_heads, PAGE, head_dim)
+                or exp.shape != pool.shape[:2] or not pool.is_contiguous() or not exp.is_contiguous()
+                or pool.device != device or exp.device != device):
+            raise KernelError(f"{what} takes e4m3 pages [pages, {kv_heads}, {PAGE}, {head_dim}] and their int8 exponents [pages, "
+                              f"{kv_heads}], contiguous, on the device of the other tensors")
+    if k_pool.shape[0] != v_pool.shape[0]:
+        raise KernelError(f"{what}: keys and values have {k_pool.shape[0]} and {v_pool.shape[0]} pages")
+    if not q8_supports(head_dim):
+        raise KernelError(f"{what} takes head sizes that are multiples of 16 up to 256, got {head_dim}")
+
+
+def _check_fused_q8(fused, batch, rope, kv_heads: int, q_per_kv: int, head_dim: int, what: str) -> int:
+    """The pairs that ``rope`` rotates, after a look at what the kernels take for granted."""
+    if not fused.is_cuda or fused.dtype != torch.bfloat16 or not fused.is_contiguous():
+        raise KernelError(f"{what} takes a contiguous bfloat16 projection on a CUDA device")
+    n = batch.n_tokens
+    if tuple(fused.shape) != (n, kv_heads * (q_per_kv + 2) * head_dim):
+        raise KernelError(f"{what}: the projection has shape {tuple(fused.shape)}, expected "
+                          f"{(n, kv_heads * (q_per_kv + 2) * head_dim)}")
+    if rope is None:
+        return 0
+    for t in rope:
+        if t.dtype != torch.float32 or t.device != fused.device or not t.is_contiguous() or t.dim() != 2 or t.shape[0] != n:
+            raise KernelError(f"{what}: cosines and sines must be contiguous float32 tensors [tokens, pairs] on the projection's device")
+    if rope[0].shape != rope[1].shape or 2 * rope[0].shape[1] > head_dim:
+        raise KernelError(f"{what}: {rope[0].shape[1]} and {rope[1].shape[1]} pairs do not fit a head of {head_dim}")
+    return rope[0].shape[1]
+
+
+def _check_slopes(slopes, heads: int, device, what: str) -> None:
+    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != heads or slopes.device != device
+                               or not slopes.is_contiguous()):
+        raise KernelError(f"{what}: slopes must be {heads} contiguous float32 numbers on the device of the other tensors")
+
+
+def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
+                          batch: StepBatchC, kv_heads: int, q_per_kv: int, head_dim: int, write_cache: bool = True, rope=None,
+                          interleaved: bool = False) -> torch.Tensor:
+    """``split_rotate_store`` for a cache in 8 bits: rotated queries [tokens, heads, head_dim] in bfloat16, and keys (rotated, not
+    rounded in between) and values as codes. A page that gets its first token takes the exponent that its new rows need (the smallest
+    e with max |x| <= 448 * 2^e); one with earlier tokens keeps its own unless the rows need a larger one, to which the earlier
+    codes are then rounded again. What is infinite or no number is held as no number. bfloat16."""
+    what = "split_rotate_store_q8"
+    pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
+    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.device, what)
+    cos, sin = rope if rope is not None else (None, None)
+    q = torch.empty((fused.shape[0], kv_heads * q_per_kv, head_dim), dtype=fused.dtype, device=fused.device)
+    with _on_device(fused):
+        _check(lib().ptb_store_q8(_ptr(fused), _ptr(q), *((_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp)) if write_cache
+                                                          else (None, None, None, None)), k_pool.shape[0], ctypes.byref(batch),
+                                  _ptr(cos), _ptr(sin), pairs, 1 if interleaved else 0, kv_heads, q_per_kv, head_dim,
+                                  _ptr(error_flag(fused.device)), _stream(fused)), what)
+    return q
+
+
+def unpack_pages_q8(k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor, ids: torch.Tensor):
+    """The pages that ``ids`` (int32, on the device) names as bfloat16 values, keys and values: [len(ids), kv_heads, PAGE, head_dim]
+    each. A page out of range reads as zeros and raises the device's error flag."""
+    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or not ids.is_cuda or k_pool.dim() != 4:
+        raise KernelError("unpack_pages_q8 takes pages of one cache entry and a contiguous int32 list of page numbers on the device")
+    kv_heads, head_dim = k_pool.shape[1], k_pool.shape[3]
+    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, ids.device, "unpack_pages_q8")
+    out = torch.empty((2, ids.numel(), kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device)
+    with _on_device(ids):
+        _check(lib().ptb_unpack_q8(_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(ids), None, None,
+                                   ids.numel(), 0, _ptr(out[0]), _ptr(out[1]), kv_heads, head_dim, head_dim,
+                                   _ptr(error_flag(ids.device)), _stream(ids)), "unpack_pages_q8")
+    return out[0], out[1]
+
+
+def _q8_parts(L, tiles: int, kv_heads: int, rows: int, head_dim: int, n_splits: int, device):
+    floats = L.ptb_attention_q8_floats(tiles, kv_heads, rows, head_dim, n_splits) if n_splits > 1 else 0
+    return (torch.empty(floats, dtype=torch.float32, device=device) if floats else None), floats
+
+
+def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
+                        batch: StepBatchC, rope, slopes: Optional[torch.Tensor], kv_heads: int, q_per_kv: int, head_dim: int,
+                        scale: float, window: int = 0, write_cache: bool = True, interleaved: bool = False, n_splits: int = 0,
+                        max_pages: int = 0) -> torch.Tensor:
+    """The attention of a step of single tokens over a cache in 8 bits: rotate the tokens' queries and keys, append key and value
+    to their pages (as ``split_rotate_store_q8`` does), attend. ``n_splits`` blocks share a sequence's pages (0: chosen from the
+    sizes and ``max_pages``, the most pages that a sequence of the step spans; by default the page table's width). At most 128
+    query heads a K/V head; head sizes are multiples of 16 up to 256. Returns [tokens, heads * head_dim]."""
+    what = "attention_decode_q8"
+    pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
+    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.device, what)
+    heads = kv_heads * q_per_kv
+    _check_slopes(slopes, heads, fused.device, what)
+    n = batch.n_seqs
+    if batch.n_tokens != n or q_per_kv > Q8_MAX_HEADS or window < 0 or n_splits < 0:
+        raise KernelError(f"{what} takes one token a sequence and at most {Q8_MAX_HEADS} query heads a K/V head")
+    cos, sin = rope if rope is not None else (None, None)
+    L = lib()
+    if n_splits == 0:
+        pages = max_pages or batch.pages_stride
+        if window:
+            pages = min(pages, window // PAGE + 2)
+        with _on_device(fused):
+            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages)
+    parts, floats = _q8_parts(L, n, kv_heads, q_per_kv, head_dim, n_splits, fused.device)
+    out = torch.empty((n, heads * head_dim), dtype=fused.dtype, device=fused.device)
+    with _on_device(fused):
+        _check(L.ptb_attention_decode_q8(_ptr(fused), _ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(out),
+                                         ctypes.byref(batch), _ptr(cos), _ptr(sin), pairs, 1 if interleaved else 0, _ptr(slopes),
+                                         heads, kv_heads, head_dim, ctypes.c_float(scale), int(window), 1 if write_cache else 0,
+                                         n_splits, _ptr(parts), ctypes.c_longlong(floats), _ptr(error_flag(fused.device)),
+                                         _stream(fused)), what)
+    return out
+
+
+def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
+                 batch: StepBatchC, tile_seq: torch.Tensor, tile_q0: torch.Tensor, n_tiles: int, tile_tokens: int,
+                 slopes: Optional[torch.Tensor], kv_heads: int, scale: float, window: int = 0, n_pages: int = 0) -> torch.Tensor:
+    """Causal attention of prompts and chunks over a cache in 8 bits that holds their keys and values already. ``q`` [tokens, heads,
+    head_dim] bfloat16; tiles of ``tile_tokens`` consecutive new tokens as for the other prompt kernels. ``n_pages``: the pages that the
+    step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of 64 or 128 take their
+    pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. Returns [tokens, heads * head_dim]."""
+    what = "attention_q8"
+    if not q.is_cuda or q.dtype != torch.bfloat16 or q.dim() != 3 or not q.is_contiguous() or q.shape[0] != batch.n_tokens:
+        raise KernelError(f"{what} takes contiguous bfloat16 queries [tokens, heads, head_dim] of the step's tokens")
+    n, heads, head_dim = q.shape
+    if heads % kv_heads or window < 0:
+        raise KernelError(f"{what}: {heads} heads on {kv_heads} K/V heads, window {window}")
+    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, q.device, what)
+    _check_slopes(slopes, heads, q.device, what)
+    for t in (tile_seq, tile_q0):
+        if t.dtype != torch.int32 or t.numel() < n_tiles or t.device != q.device or not t.is_contiguous():
+            raise KernelError(f"{what}: tile lists must be contiguous int32 tensors of {n_tiles} tiles on the queries' device")
+    L = lib()
+    if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and attention_tc_supports(head_dim) and not (slopes is not None and window):
+        return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
+                                      window, n_pages)
+    rows = tile_tokens * (heads // kv_heads)
+    with _on_device(q):
+        n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, min(batch.pages_stride, n_pages or batch.pages_stride))
+        parts, floats = _q8_parts(L, n_tiles, kv_heads, rows, head_dim, n_splits, q.device)
+        out = torch.empty((n, heads * head_dim), dtype=q.dtype, device=q.device)
+        _check(L.ptb_attention_q8(_ptr(q), _ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(out),
+                                  ctypes.byref(batch), _ptr(tile_seq), _ptr(tile_q0), n_tiles, tile_tokens, _ptr(slopes), heads, kv_heads,
+                                  head_dim, ctypes.c_float(scale), int(window), n_splits, _ptr(parts), ctypes.c_longlong(floats),
+                                  _ptr(error_flag(q.device)), _stream(q)), what)
+    return out
+
+
+def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale, window, n_pages):
+    head_dim, device = q.shape[2], q.device
+    # sizes in steps of an eighth: the prompt kernel keeps a tensor map for every size of pool
+    step = max(1, 1 << max(0, n_pages.bit_length() - 3))
+    room = (n_pages + step - 1) // step * step
+    tmp = torch.empty((2, room, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=device)
+    table = torch.empty((batch.n_seqs, batch.pages_stride), dtype=torch.int32, device=device)
+    with _on_device(q):
+        _check(lib().ptb_unpack_q8(_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], None, ctypes.byref(batch),
+                                   _ptr(table), n_pages, int(window), _ptr(tmp[0]), _ptr(tmp[1]), kv_heads, head_dim, head_dim,
+                                   _ptr(error_flag(device)), _stream(q)), "attention_q8 (pages)")
+        unpacked = StepBatchC.from_buffer_copy(batch)
+        unpacked.pages = table.data_ptr()
+        if slopes is not None:
+            return attention_tc(q, tmp[0], tmp[1], unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, slopes)
+        return attention_tc_extras(q, tmp[0], tmp[1], unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
+
+
+def copy_pages(pools, src, dst, out=None):
+    """Pages ``src[i]`` to ``dst[i]`` in every tensor of ``pools`` ([entries, pages, ...], contiguous, of any type; at most eight),
+    or into the tensors ``out`` of the same types and page shapes (other storage, with pages of its own number). ``src`` and ``dst``:
+    int32 NumPy arrays or sequences of page numbers; a source may be named often, a target once, and within one storage no page
+    may be both. One launch for up to 960 pairs. Returns the tensors written to."""
+    into = list(pools) if out is None else list(out)
+    src, dst = np.ascontiguousarray(src, dtype=np.int32), np.ascontiguousarray(dst, dtype=np.int32)
+    k = len(pools)
+    if k == 0 or k > 8 or len(into) != k or src.ndim != 1 or src.shape != dst.shape:
+        raise KernelError("copy_pages takes one to eight tensors, as many targets and one target page for each source page")
+    args = []
+    for a, b in zip(pools, into):
+        if (a.dim() < 2 or not a.is_cuda or b.device != a.device or a.device != pools[0].device or a.dtype != b.dtype or a.shape[0] != b.shape[0]
+                or a.shape[2:] != b.shape[2:] or a.shape[1] != pools[0].shape[1] or b.shape[1] != into[0].shape[1]
+                or not a.is_contiguous() or not b.is_contiguous()):
+            raise KernelError("copy_pages takes contiguous tensors [entries, pages, ...] on one CUDA device, all with the same number of "
+                              "pages, and targets that differ in that number only")
+        page = a.element_size() * math.prod(a.shape[2:])
+        args.append((a.data_ptr(), b.data_ptr(), a.shape[1] * page, b.shape[1] * page, page, a.shape[0]))
+    ranges = [(p, p + n * e, q, q + m * e) for p, q, n, m, _, e in args]
+    if out is not None and any(lo < hi2 and lo2 < hi for lo, hi, _, _ in ranges for _, _, lo2, hi2 in ranges if lo < hi and lo2 < hi2):
+        raise KernelError("copy_pages: the targets lie in the sources' memory")
+    col = list(zip(*args))
+    pointers, numbers = ctypes.c_void_p * k, ctypes.c_longlong * k
+    t = pools[0]
+    with _on_device(t):
+        _check(lib().ptb_copy_pages(pointers(*col[0]), pointers(*col[1]), numbers(*col[2]), numbers(*col[3]), numbers(*col[4]),
+                                    (ctypes.c_int * k)(*col[5]), k, ctypes.c_void_p(src.ctypes.data), ctypes.c_void_p(dst.ctypes.data),
+                                    ctypes.c_longlong(src.size), t.shape[1], into[0].shape[1], _stream(t)), "copy_pages")
+    return into
