@@ -497,22 +497,30 @@ _error_flags = {}
 TC_TILE_TOKENS = 128  # ptb_attention_tc_tile_tokens()
 
 
+def _with_index(device) -> torch.device:
+    """``device`` by its number: "cuda" is the current one."""
+    device = torch.device(device)
+    return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
+
+
 def error_flag(device) -> torch.Tensor:
     """Device int32 word that kernels with bounded waits raise when a wait runs out."""
-    device = torch.device(device)
+    device = _with_index(device)
     if device not in _error_flags:
         _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
     return _error_flags[device]
 
 
 def check_device_errors(device) -> None:
-    """Raise if a kernel has reported that one of its bounded waits ran out (synchronises)."""
-    device = torch.device(device)
+    """Raise if a kernel has reported that one of its bounded waits ran out, or a page number that is none (synchronises)."""
+    device = _with_index(device)
     flag = _error_flags.get(device)
     if flag is not None:
         code = int(flag.item())
         if code != 0:
             flag.zero_()
+            if code == 21:
+                raise KernelError("a page table or list named a page that the cache does not have: the results are void")
             raise KernelError(f"a kernel gave up waiting inside its pipeline (code {code}): its results are void")
 
 
