@@ -18,7 +18,8 @@ class CacheError(RuntimeError):
 
 
 class IdPool:
-    """Integer ids 0 .. capacity-1, handed out lowest first and taken back."""
+    """Integer ids 0 .. capacity-1, handed out lowest first and taken back. An id that is out may be shared: it goes back to the
+    free ones when every holder has given it back."""
 
     def __init__(self, capacity: int, what: str):
         if capacity < 0:
@@ -27,7 +28,7 @@ class IdPool:
         self.what = what
         self._free: List[int] = list(range(capacity))
         heapq.heapify(self._free)
-        self._held = [False] * capacity
+        self._held = [0] * capacity     # holders of each id
 
     @property
     def available(self) -> int:
@@ -46,21 +47,58 @@ class IdPool:
         for i in out:
             if self._held[i]:
                 raise CacheError(f"{self.what} {i} was in the free list while held")  # never expected
-            self._held[i] = True
+            self._held[i] = 1
         return out
 
-    def give_back(self, ids) -> None:
-        ids = list(ids)
+    def _must_be_out(self, ids) -> None:
         for i in ids:
             if not (0 <= i < self.capacity):
                 raise CacheError(f"{self.what} {i} is outside 0..{self.capacity - 1}")
             if not self._held[i]:
                 raise CacheError(f"{self.what} {i} is freed twice (or was never given out)")
+
+    def share(self, ids) -> None:
+        """One more holder for each of ``ids``, which are out."""
+        ids = list(ids)
+        self._must_be_out(ids)
+        for i in ids:
+            self._held[i] += 1
+
+    def holders(self, i: int) -> int:
+        return self._held[i]
+
+    def give_back(self, ids) -> None:
+        ids = list(ids)
+        self._must_be_out(ids)
         if len(set(ids)) != len(ids):
             raise CacheError(f"a {self.what} is named twice in one release: {ids}")
         for i in ids:
-            self._held[i] = False
+            self._held[i] -= 1
+            if self._held[i] == 0:
+                heapq.heappush(self._free, i)
+
+    def renumber(self, capacity: int) -> Dict[int, int]:
+        """Give the ids that are out new numbers 0 .. in_use-1 in a pool of ``capacity``: those below in_use keep theirs, the others
+        take the lowest free ones. Returns {old: new} of the ids that changed."""
+        n = self.in_use
+        if capacity < n:
+            raise CacheFull(f"{n} {self.what}s are out, more than a capacity of {capacity}")
+        holes = [i for i in range(n) if not self._held[i]]
+        moved = dict(zip((i for i in range(n, self.capacity) if self._held[i]), holes))
+        held = self._held[:n]
+        for old, new in moved.items():
+            held[new] = self._held[old]
+        self.capacity = capacity
+        self._held = held + [0] * (capacity - n)
+        self._free = list(range(n, capacity))      # sorted: a heap
+        return moved
+
+    def grow(self, capacity: int) -> None:
+        """More ids, behind those that there are."""
+        for i in range(self.capacity, capacity):
+            self._held.append(0)
             heapq.heappush(self._free, i)
+        self.capacity = max(self.capacity, capacity)
 
     def check(self) -> None:
         """Every id is either free or held, exactly once."""

@@ -62,6 +62,8 @@ class RunGenerationCommand(BaseCommand):
         p.add_argument("--greedy", action="store_true", help="argmax instead of sampling")
         p.add_argument("--fp32", action="store_true", help="true 32-bit path instead of bfloat16")
         p.add_argument("--batch_size", type=int, default=64)
+        p.add_argument("--cache_dtype", default="auto", choices=["auto", "float8_e4m3fn"], help="how keys and values are held")
+        p.add_argument("--share_prompts", action="store_true", help="run a prompt once for all of its returned sequences")
         p.set_defaults(func=RunGenerationCommand)
 
     def __init__(self, args):
@@ -96,7 +98,7 @@ class RunGenerationCommand(BaseCommand):
             else:
                 raise SystemExit(f"--stop_token {a.stop_token!r} is neither a token id nor a known token")
         kw = dict(max_new_tokens=a.length, repetition_penalty=a.repetition_penalty, eos_token_id=eos,
-                  max_batch_size=a.batch_size)
+                  max_batch_size=a.batch_size, cache_dtype=a.cache_dtype, share_prompts=a.share_prompts)
         if a.greedy:
             out = model.generate(prompts, do_sample=False, **kw)
         else:

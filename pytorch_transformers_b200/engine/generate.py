@@ -23,7 +23,8 @@ class Stepper(Protocol):
     def open(self) -> int: ...
     def close(self, slot: int) -> None: ...
     def step(self, slots: Sequence[int], token_lists: Sequence[Sequence[int]]): ...
-    # optional: prepare(slots) builds the next step of one token each ahead of time;
+    # optional: fork(slot) -> slot: another sequence with the same past (needed where prompts are shared)
+    #           prepare(slots) builds the next step of one token each ahead of time;
     #           step_ahead(slots, device_tokens) runs that step with token ids that only the device knows yet
     #           (returns None if it cannot: the loop then waits for the tokens and calls step)
 
@@ -53,12 +54,16 @@ def run_generation(stepper: Stepper, selector: Selector, prompts: Sequence[Seque
                    options: GenerationConfig, budget: int, max_batch: int,
                    on_token: Optional[Callable[[int, int], None]] = None,
                    keep_logits: bool = False,
-                   on_step: Optional[Callable[[dict], None]] = None) -> List[RequestResult]:
+                   on_step: Optional[Callable[[dict], None]] = None,
+                   same_as: Optional[Sequence[int]] = None) -> List[RequestResult]:
     """Generate up to ``budget`` tokens for every prompt; returns results in the prompts' order.
 
     ``on_token(request_index, token)`` is called for every new token as it is chosen, and
     ``on_step({request_index: token})`` once per step with all of the step's new tokens (the
-    reference's streamer gets a step's tokens in one call, utils.py:3287-3288)."""
+    reference's streamer gets a step's tokens in one call, utils.py:3287-3288).
+
+    ``same_as[i]``: the number of a request with the same prompt as request i (itself, if it is the first of them). A batch runs such a
+    prompt once and forks its sequence for the others (the stepper's ``fork``)."""
     for i, p in enumerate(prompts):
         if len(p) == 0:
             raise ValueError(f"prompt {i} is empty: a sequence needs at least one token to start from")
@@ -74,11 +79,26 @@ def run_generation(stepper: Stepper, selector: Selector, prompts: Sequence[Seque
         held = set()
         live = []
         try:
+            leaders = {}                          # the first request of the batch with each prompt -> its row of the step
             for r in batch:
-                slot = stepper.open()
-                held.add(slot)
-                live.append((r, slot))
+                key = r if same_as is None else same_as[r]
+                if key not in leaders:
+                    slot = stepper.open()
+                    held.add(slot)
+                    leaders[key] = len(live)
+                    live.append((r, slot))
             logits = stepper.step([s for _, s in live], [results[r].prompt for r, _ in live])
+            if len(live) < len(batch):
+                rows = [leaders[same_as[r]] for r in batch]
+                first, live = live, []
+                for r, row in zip(batch, rows):
+                    if first[row][0] == r:
+                        live.append(first[row])
+                    else:
+                        slot = stepper.fork(first[row][1])
+                        held.add(slot)
+                        live.append((r, slot))
+                logits = logits[rows]
             for t in range(budget):
                 req_ids = [r for r, _ in live]
                 slots = [s for _, s in live]

@@ -218,8 +218,9 @@ class CausalLM:
                           mixer.state_need() if mixer else None))
         return needs
 
-    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None) -> Cache:
-        return Cache(self.cache_needs(), max_tokens, self.dtype, self.device, max_slots=max_slots)
+    def new_cache(self, max_tokens: int, max_slots: Optional[int] = None, kv_dtype: Optional[torch.dtype] = None) -> Cache:
+        """``kv_dtype=torch.float8_e4m3fn``: keys and values in 8 bits (cache/paged.py), where every mixer takes them."""
+        return Cache(self.cache_needs(), max_tokens, self.dtype, self.device, max_slots=max_slots, kv_dtype=kv_dtype)
 
     # ------------------------------------------------------------------ the step
     def step(self, cache: Cache, slots: Sequence[int], token_lists: Sequence[Sequence[int]],

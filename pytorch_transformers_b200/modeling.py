@@ -10,7 +10,7 @@ the safetensors weights (src/transformers/modeling_utils.py:3138-4368 in the ref
 token lists; ``max_new_tokens``, ``max_length``, ``min_new_tokens``, ``do_sample``,
 ``temperature``, ``top_k``, ``top_p``, ``min_p``, ``repetition_penalty``,
 ``num_return_sequences``, ``eos_token_id``, ``pad_token_id``, ``output_logits``,
-``return_dict_in_generate``, ``streamer``. Everything runs on one CUDA device through the
+``return_dict_in_generate``, ``streamer``; its own are ``cache_dtype`` and ``share_prompts``. Everything runs on one CUDA device through the
 library's own kernels.
 """
 from __future__ import annotations
@@ -55,6 +55,18 @@ def resolve_dtype(dtype, config: Optional[ModelConfig] = None, folder: Optional[
         raise ValueError(f"dtype must be bfloat16 or float32, got {dtype!r}") from None
 
 
+_CACHE_DTYPES = {"float8_e4m3fn": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn, torch.float8_e4m3fn: torch.float8_e4m3fn}
+
+
+def resolve_cache_dtype(cache_dtype, dtype: torch.dtype) -> Optional[torch.dtype]:
+    """The cache's own dtype for keys and values, or None for the model's (None, "auto" or its name)."""
+    if cache_dtype in (None, "auto") or _DTYPES.get(cache_dtype) == dtype:
+        return None
+    if cache_dtype not in _CACHE_DTYPES:
+        raise ValueError(f"cache_dtype must be the model's dtype or float8_e4m3fn, got {cache_dtype!r}")
+    return _CACHE_DTYPES[cache_dtype]
+
+
 @dataclasses.dataclass
 class GenerateOutput:
     """``sequences``: prompt + new tokens per request (a padded LongTensor if the input was one);
@@ -78,6 +90,9 @@ class _CacheStepper:
 
     def close(self, slot: int) -> None:
         self.cache.close(slot)
+
+    def fork(self, slot: int) -> int:
+        return self.cache.fork(slot)
 
     def prepare(self, slots) -> None:
         self.model.prepare_next(self.cache, slots)
@@ -148,20 +163,24 @@ class PreTrainedCausalLM(CausalLM):
         return model
 
     # ------------------------------------------------------------------ generation
-    def _ensure_cache(self, max_tokens: int) -> Cache:
+    def _ensure_cache(self, max_tokens: int, kv_dtype: Optional[torch.dtype] = None) -> Cache:
         cache = getattr(self, "_cache", None)
-        if cache is None or cache.max_tokens < max_tokens or cache.records:
+        if cache is None or cache.max_tokens < max_tokens or cache.records or cache.kv_dtype != kv_dtype:
             if cache is not None and cache.records:
                 cache = None  # somebody holds sequences in it: leave it alone, use a private one
             self._cache = None
-            cache = self.new_cache(max_tokens)
+            cache = self.new_cache(max_tokens, kv_dtype=kv_dtype)
             self._cache = cache
         return cache
 
     @torch.no_grad()
     def generate(self, inputs=None, generation_config: Optional[GenerationConfig] = None, *, input_ids=None,
                  attention_mask=None, streamer=None, max_batch_size: int = 64, max_step_tokens: int = 16384,
-                 on_token: Optional[Callable[[int, int], None]] = None, **kwargs):
+                 on_token: Optional[Callable[[int, int], None]] = None, cache_dtype=None, share_prompts: bool = False, **kwargs):
+        """``cache_dtype``: "float8_e4m3fn" holds keys and values in 8 bits (by default in the model's dtype). ``share_prompts``:
+        with ``num_return_sequences`` > 1 a prompt runs once for all of its sequences of a batch, which share its whole pages
+        (by default each runs its own, as one row of the step's batch)."""
+        kv_dtype = resolve_cache_dtype(cache_dtype, self.dtype)
         if inputs is None:
             inputs = input_ids
         if inputs is None:
@@ -205,7 +224,7 @@ class PreTrainedCausalLM(CausalLM):
         need = 0
         for i in range(0, len(expanded), max_batch):
             need = max(need, sum((len(p) + budget + PAGE - 1) // PAGE * PAGE for p in expanded[i:i + max_batch]))
-        cache = self._ensure_cache(need)
+        cache = self._ensure_cache(need, kv_dtype)
         selector = DeviceSelector(self.build.kernels, self.device, self.spec.vocab_size, opts, max_rows=max_batch,
                                   max_history=longest + budget)
 
@@ -234,7 +253,8 @@ class PreTrainedCausalLM(CausalLM):
 
         results = run_generation(_CacheStepper(self, cache, max_step_tokens), selector, expanded, opts, budget, max_batch,
                                  on_token=_on_token if on_token is not None else None,
-                                 keep_logits=opts.output_logits, on_step=_on_step if stream_steps else None)
+                                 keep_logits=opts.output_logits, on_step=_on_step if stream_steps else None,
+                                 same_as=[i - i % n_ret for i in range(len(expanded))] if share_prompts and n_ret > 1 else None)
         self.check_errors()
         if streamer is not None:
             if not stream_steps:

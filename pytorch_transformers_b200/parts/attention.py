@@ -81,7 +81,8 @@ class Attention(Part):
         return d
 
     def cache_need(self):
-        return CacheNeed("window" if self.window > 0 else "full", self.kv_heads, self.head_dim, self.window)
+        return CacheNeed("window" if self.window > 0 else "full", self.kv_heads, self.head_dim, self.window,
+                         eight_bit=self.head_dim % 16 == 0)
 
     def state_need(self):
         return None
@@ -97,7 +98,8 @@ class Attention(Part):
             return False
         lengths = (p + n for p, n in zip(ctx.past, ctx.new))
         keys = sum(min(t, self.window) if self.window else t for t in lengths)
-        return self.build.kernels.decode_attention_fits_beside(keys * self.kv_heads * self.head_dim * 2 * 2, self.head_dim)
+        size = 2 if getattr(getattr(ctx, "cache", None), "kv_dtype", None) is None else 1
+        return self.build.kernels.decode_attention_fits_beside(keys * self.kv_heads * self.head_dim * 2 * size, self.head_dim)
 
     fuses_add = True
 
@@ -112,6 +114,10 @@ class Attention(Part):
         slopes = self.position.score_bias() if self.position is not None else None
         inter = bool(getattr(self.position, "interleaved", False))   # rotated pairs (2 i, 2 i + 1) instead of (i, i + n)
         tiles = ctx.plan(AttentionTiles.plan_key)
+        exps = ctx.cache.entry_exponents(entry.cache_entry)
+        if exps is not None:
+            o = self._attend_q8(fused, (k_pool, exps[0], v_pool, exps[1]), ctx, entry, tiles, batch, rope, slopes, inter)
+            return linear(k, o, self.p_out_weight, self.p_out_bias, add=add)
         if tiles.facts["mma_tokens"] == 1 and fused.dtype == self._bf16 and k.attention_mma_supports(self.head_dim):
             # a step of single tokens: rotation, cache write, attention and the join in one kernel
             hpk = min(self.q_per_kv, 128)
@@ -145,6 +151,22 @@ class Attention(Part):
                                      self.head_dim, write_cache=entry.writes_cache, rope=rope, interleaved=inter)
             o = self.attend(q, k_pool, v_pool, ctx, tiles, batch, slopes)
         return linear(k, o, self.p_out_weight, self.p_out_bias, add=add)
+
+    def _attend_q8(self, fused, cache, ctx, entry, tiles, batch, rope, slopes, interleaved):
+        """Over a cache in 8 bits: one kernel for a step of single tokens, else queries, keys and values apart and then the
+        attention of the step's tiles."""
+        k = self.build.kernels
+        tokens = tiles.facts["mma_tokens"]
+        if tokens == 1 and self.q_per_kv <= k.Q8_MAX_HEADS:
+            return k.attention_decode_q8(fused, *cache, batch, rope, slopes, self.kv_heads, self.q_per_kv, self.head_dim, self.scale,
+                                         window=self.window, write_cache=entry.writes_cache, interleaved=interleaved,
+                                         max_pages=ctx.pages_hint)
+        q = k.split_rotate_store_q8(fused, *cache, batch, self.kv_heads, self.q_per_kv, self.head_dim, write_cache=entry.writes_cache,
+                                    rope=rope, interleaved=interleaved)
+        first = [max(0, p - self.window + 1) // k.PAGE if self.window > 0 else 0 for p in ctx.past]
+        pages = sum((p + n + k.PAGE - 1) // k.PAGE - f for p, n, f in zip(ctx.past, ctx.new, first))
+        return k.attention_q8(q, *cache, batch, tiles.dev["mtile_seq"], tiles.dev["mtile_q0"], tiles.facts["n_mma_tiles"], tokens, slopes,
+                              self.kv_heads, self.scale, window=self.window, n_pages=pages)
 
     def _decode_splits(self, ctx, hpk):
         """Blocks per (sequence, head chunk) for steps of single tokens: up to about two blocks on

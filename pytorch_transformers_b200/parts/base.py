@@ -141,13 +141,15 @@ class CacheNeed:
     and values of the sequence) or ``"window"`` (the last ``window`` of them). ``v_head_dim``: size of a
     value row if it differs from a key row's; 0 for an entry that keeps one row per token only (a mixer
     whose values are part of its keys: latent attention). ``keep_first``: a ``window`` entry whose sequences' first
-    ``keep_first`` positions stay readable for good (their pages are never given back)."""
+    ``keep_first`` positions stay readable for good (their pages are never given back). ``eight_bit``: the mixer can
+    read and write pages held as e4m3 codes with exponents (``Cache(kv_dtype=torch.float8_e4m3fn)``)."""
     kind: str
     kv_heads: int
     head_dim: int
     window: int = 0
     v_head_dim: Optional[int] = None
     keep_first: int = 0
+    eight_bit: bool = False
 
 
 @dataclasses.dataclass(frozen=True)
