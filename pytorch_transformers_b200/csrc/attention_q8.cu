@@ -7,29 +7,37 @@
 // launch; a block's rows are the query heads of one K/V head), and prompts or chunks whose queries are given (rows: tokens x heads).
 //
 // What bounds it is the codes' way from memory, so everything is laid out for that. A code becomes a float16 number exactly
-// (cvt.rn.f16x2.e4m3x2), and mma.m16n8k16 takes float16 operands; queries are float16 numbers of 11 bits after their row is
+// (cvt.rn.f16x2.e4m3x2), and mma.m16n8k16 takes float16 operands, the codes as its larger one: S^T = K Q^T with 16 keys by 8 rows, and
+// O^T = V^T P^T with 16 entries by 8 rows, since few query heads read a K/V head (with 16 rows by 8 keys, four heads of 128 on each K/V head
+// waste three quarters of the products and twice the registers). The weights' way from one to the other is a transposition of 8 x 8 (movmatrix). Queries are float16 numbers of 11 bits after their row is
 // brought to [1, 2) by a power of two, softmax weights float16 of 11 bits (bfloat16 ones of 8 would cost as much error as the
 // output's own rounding). Sums, maxima and the output are float32.
 //
-// A warp has 16 keys at a time to itself: it copies them (16 rows of D codes, keys and values, contiguous in the page)
-// with cp.async into a ring of its own, so that no warp waits for another before the end. Which key and which entry an index of the
+// Pages land whole, keys and values, in rings that the tensor memory accelerator fills (2 requests a page: with boxes of 16 or
+// 32 rows, asked for by the warp that reads them or by one warp for all, the requests alone took 175 of 200 us where memory allows
+// 150). The warps of a ring take a share of a page's keys each, for one part of the rows or another; whoever is the last to have
+// read a page asks for the next one into its place. So no warp waits for another, but through a ring of pages, before the end. Which key and which entry an index of the
 // matrix instruction stands for is free as long as both operands agree: a thread's share of a key's row is 16 codes in a row (a
-// 16-byte load gives four k-steps of B fragments), and its share of a value's row likewise (columns of the output are
-// named accordingly, pairs of keys are put together with byte permutes). Nothing is transposed. Rows lie in the ring
-// under an exclusive-or of their number, so that both ways of reading are free of bank conflicts.
+// 16-byte load gives four k-steps of fragments), and its share of a value's row likewise (columns of the output are
+// named accordingly, pairs of keys are put together with byte permutes). Nothing is transposed. The accelerator's swizzle and
+// an order of keys within eight (kappa) keep both ways of reading free of bank conflicts.
 //
 // Pages have exponents of their own: keys' go into the factor of a page's scores; values' are the unit of the float32
 // output, which is multiplied by a power of two (exactly) where the unit changes. The unit stays within 2^60 of the largest exponent
 // seen, so that the output cannot overflow in small units; smaller pages' weights are scaled instead, which no number notices.
 // The running maximum moves only when a score exceeds it by 2^8 (one vote a tile instead of shuffles for each row).
-#include "mma_common.cuh"
+#include <cooperative_groups.h>
+
 #include "q8.cuh"
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int TILE = 16;              // keys of a step of a warp
 constexpr float MOVE_LOG2 = 8.f;      // float16 weights go up to 2^8 then
-constexpr int UNIT_RANGE = 60;
+constexpr int UNIT_RANGE = 60, UNIT_SLACK = 3;
+constexpr int MAX_CLUSTER = 8;
 
 struct AttnQ8 {
   const __nv_bfloat16* rows;           // FUSED: the projection; else queries [tokens, heads, dim]
@@ -39,96 +47,187 @@ struct AttnQ8 {
   const float *rope_cos, *rope_sin, *slopes;
   const int *tile_seq, *tile_q0;       // not FUSED
   int tile_tokens;
-  int heads, kv_heads, dim, pool_pages, rot_pairs, interleaved, write_cache, window, n_splits;
-  int row_groups, key_groups;          // warps = row_groups * key_groups
+  int heads, kv_heads, dim, pool_pages, rot_pairs, interleaved, write_cache, window;
+  int n_splits, cluster, teams;        // blocks that share a row's pages = cluster (one thread-block cluster) * teams
+  int row_groups, page_parts, rings, stages;      // warps at work = row_groups * page_parts * rings
+  int ring_bytes;                      // of shared memory before the queries
   float scale;
-  float* parts;                        // [grid x][grid y][n_splits][rows][dim + 2] where n_splits > 1
+  float* parts;                        // [grid x][grid y][teams][rows][dim + 2] where teams > 1
   int* error_flag;
 };
 
-template <int DP> struct Q8Shape {
-  static constexpr int STAGES = DP == 256 ? 2 : 4;      // 256: beside 68 KB of queries in 128 rows
-  static constexpr int STAGE_BYTES = 2 * TILE * DP;      // keys, then values
-  static constexpr int Q_PITCH = DP * 2 + 16;
+// DP: 64, 128 or 256 entries that a head of `dim` is padded to; NH: eights of rows that a warp holds (a code is unpacked once for all
+// of them).
+constexpr int WARPS = 8, MAX_STAGES = 8;
+template <int DP, int NH> struct Q8Shape {
+  static constexpr int TILE = DP == 64 ? 32 : 16;        // keys of a warp's step
+  static constexpr int BLOCKS = DP == 256 || NH == 4 ? 1 : 2;   // on an SM
+  static constexpr int STAGE_BYTES = 2 * PTB_PAGE * DP;  // a page of one K/V head: keys, then values
   static constexpr int PITCH = DP + 4;                   // floats of a row of the join
 };
 
-// where the 16-byte chunk `c` of the tile's row `key` lies: see the head of the file
+// The order of a tile's keys: column c of eight stands for key kappa(c). A quarter-warp's 16-byte reads of keys touch columns 2 t and
+// 2 t + 1, of values columns 2 t + b for four t: both sets have to lie in different banks under the copies' swizzle.
+template <int DP> __device__ __forceinline__ int kappa(int c) {
+  const int t = c >> 1;
+  if (DP == 64) return (c & 1) ? ((t & 1) + ((t & 2) << 1)) ^ 3 : (t & 1) + ((t & 2) << 1);      // 0 3 1 2 4 7 5 6
+  return (c & 1) ? ((2 * t) ^ 4) + 1 : 2 * t;                                                    // 0 5 2 7 4 1 6 3
+}
+// where the 16-byte chunk `c` of the page's row `key` lies: the 64- and 128-byte swizzles of the copies (boxes of 128 bytes side by side)
 template <int DP> __device__ __forceinline__ int place(int key, int c) {
-  if (DP == 64) {
-    const int row = key ^ ((key >> 2) & 1);
-    return row * 64 + ((c ^ (((row >> 1) & 1) << 1)) << 4);
-  }
-  return key * DP + ((c ^ ((key & 6) ^ ((key & 1) << 2))) << 4);
+  if (DP == 64) return key * 64 + ((c ^ ((key >> 1) & 3)) << 4);
+  return (c >> 3) * (PTB_PAGE * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// an 8 x 8 matrix of 16-bit numbers, a thread two of row lane / 4, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   uint32_t h;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(hi), "f"(lo));
   return h;
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+// Eighths of rows of the projection on their way (a row's own and the one that holds its pairs' other halves), and the angles of an
+// eighth, which are the same for all rows: what a lane rotates in registers once all of its loads are out.
+struct Angles {
+  float c[8], s[8];
+  int mode;      // 0: not rotated; 1: pairs within the eighth; 2: the pairs' other halves in the eighth `other`; 3: entry by entry
+  int other;
+  bool upper;
+};
+__device__ __forceinline__ Angles angles_of(int c, const float* rc, const float* rs, int P, int interleaved) {
+  Angles a;
+  const int d0 = 8 * c;
+  a.other = c;
+  a.upper = d0 >= P;
+  a.mode = d0 >= 2 * P ? 0 : interleaved ? 1 : (P & 7) == 0 ? 2 : 3;
+  if (a.mode == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d0 / 2 + i < P) a.c[i] = rc[d0 / 2 + i], a.s[i] = rs[d0 / 2 + i];
+      else a.c[i] = 1.f, a.s[i] = 0.f;
+  } else if (a.mode == 2) {
+    const int e0 = a.upper ? d0 - P : d0;
+    a.other = (a.upper ? e0 : e0 + P) / 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.c[i] = rc[e0 + i], a.s[i] = rs[e0 + i];
+  }
+  return a;
+}
+__device__ __forceinline__ void rotate8(const Angles& a, const uint4& own, const uint4& other, float (&x)[8]) {
+  unpack_bf16x8(own, x);
+  if (a.mode == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (a.c[i] != 1.f || a.s[i] != 0.f) rotate_pair(x[2 * i], x[2 * i + 1], a.c[i], a.s[i], x[2 * i], x[2 * i + 1]);
+  } else if (a.mode == 2) {
+    float y[8];
+    unpack_bf16x8(other, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float ra, rb;
+      rotate_pair(a.upper ? y[i] : x[i], a.upper ? x[i] : y[i], a.c[i], a.s[i], ra, rb);
+      x[i] = a.upper ? rb : ra;
+    }
+  }
+}
 
-// One token's key (or value) into its page, by one warp: the rule of store_q8_kernel for a page that gets one row.
-__device__ void append_row(const __nv_bfloat16* row, const float* rc, const float* rs, int P, int interleaved, uint8_t* codes, int8_t* exps,
-                           int at, int dim) {
+// One token's key (or value) into its page, by one warp: the rule of store_q8_kernel for a page that gets one row. The row's codes go to
+// `copy` as well, and the page's exponent is returned; `rose`: it is larger than before, and the earlier codes have been
+// rounded again, seen by all who read them after the block's next barrier.
+__device__ int append_row(const __nv_bfloat16* row, const float* rc, const float* rs, int P, int interleaved, uint8_t* codes, int8_t* exps,
+                          int at, int dim, unsigned char* copy, bool& rose) {
   const int lane = threadIdx.x & 31;
+  const int old = at > 0 ? int(__ldcg(reinterpret_cast<const signed char*>(exps))) : Q8_EXP_MIN;
   float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
   if (lane * 8 < dim) {
     load_rotated8(row, lane, rc, rs, P, interleaved, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_abs(x[e]));
   }
-  int e = q8_exponent(warp_max(most));
-  if (at > 0) {
-    const int old = __ldcg(reinterpret_cast<const signed char*>(exps));
-    e = max(e, old);
-    if (e > old) {
-      const float down = power_of_two(max(old - e, -126));
-      for (int i = lane; i < at * dim / 16; i += 32) {
-        uint4 w = __ldcg(reinterpret_cast<const uint4*>(codes) + i);
-        uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+  const int e = max(q8_exponent(warp_max(most)), old);
+  rose = at > 0 && e > old;
+  if (rose) {
+    const float down = power_of_two(max(old - e, -126));
+    for (int i = lane; i < at * dim / 16; i += 32) {
+      uint4 w = __ldcg(reinterpret_cast<const uint4*>(codes) + i);
+      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float f[4];
-          q8_unpack4(u[k], f);
-          u[k] = q8_pack4(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
-        }
-        reinterpret_cast<uint4*>(codes)[i] = w;
+      for (int k = 0; k < 4; ++k) {
+        float f[4];
+        q8_unpack4(u[k], f);
+        u[k] = q8_pack4(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
       }
+      reinterpret_cast<uint4*>(codes)[i] = w;
     }
   }
-  __syncwarp();
   const float by = power_of_two(-e);
-  if (lane * 8 < dim)
-    *reinterpret_cast<uint2*>(codes + size_t(at) * dim + lane * 8) =
-        make_uint2(q8_pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), q8_pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+  if (lane * 8 < dim) {
+    const uint2 w = make_uint2(q8_pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), q8_pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
+    *reinterpret_cast<uint2*>(codes + size_t(at) * dim + lane * 8) = w;
+    *reinterpret_cast<uint2*>(copy + lane * 8) = w;
+  }
   if (lane == 0) *exps = int8_t(e);
+  if (rose) {      // the accelerator reads them next
+    __threadfence();
+    asm volatile("fence.proxy.async;\n" ::: "memory");
+  }
+  return e;
 }
 
-// MT: tiles of 16 rows that a warp holds; a code is unpacked once for all of them.
-template <int DP, int MT, bool FUSED>
-__global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) attention_q8_kernel(StepBatch sb, AttnQ8 p) {
-  using Shape = Q8Shape<DP>;
-  constexpr int STAGES = Shape::STAGES, KS = DP / 16, NT = DP / 8;       // k-steps of a score, 8-column tiles of the output
-  constexpr bool Q_REGS = MT * DP <= 128;
-  pdl_entry();
-  extern __shared__ __align__(128) unsigned char smem[];
+template <int DP, int NH, bool FUSED>
+__global__ void __launch_bounds__(WARPS * 32, Q8Shape<DP, NH>::BLOCKS)
+attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using Shape = Q8Shape<DP, NH>;
+  constexpr int TILE = Shape::TILE, KS = DP / 16, ST = TILE / 16;      // steps of 16 entries, of 16 keys
+  constexpr bool Q_REGS = NH * DP <= 128;      // else the queries' fragments come from shared memory, tile by tile
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t bars[WARPS][MAX_STAGES];      // ring, stage: the page has landed
+  __shared__ int readers[WARPS][MAX_STAGES];                      // warps that have read it
+  __shared__ __align__(16) unsigned char new_rows[2][DP];      // FUSED: the new token's codes, the page's exponents and whether one rose
+  __shared__ int new_exp[2], new_rose[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
   const int g4 = lane >> 2, t4 = lane & 3;
-  const int rg = warp % p.row_groups, kg = warp / p.row_groups;
-  const int rows_pad = p.row_groups * 16 * MT;
-  unsigned char* q_s = smem;
-  int* row_exp = reinterpret_cast<int*>(q_s + size_t(rows_pad) * Shape::Q_PITCH);
-  unsigned char* rings = reinterpret_cast<unsigned char*>(row_exp + rows_pad);
-  unsigned char* ring = rings + size_t(warp) * STAGES * Shape::STAGE_BYTES;
+  // this warp's eights of rows, its part of every page that lands in its ring, and the ring
+  const int rg = warp % p.row_groups, part = warp / p.row_groups % p.page_parts, ring_no = warp / (p.row_groups * p.page_parts);
+  const bool idle = ring_no >= p.rings;
+  const int key_groups = p.page_parts * p.rings, kg = ring_no * p.page_parts + part;
+  const int rows_pad = p.row_groups * 8 * NH;
+  // shared memory, by offsets from a base of 1,024 bytes: rings (later the join), queries, their exponents, maxima and sums
+  unsigned char* smem = smem_dyn + ((1024 - (smem_u32(smem_dyn) & 1023)) & 1023);
+  const int ring = ring_no * p.stages * Shape::STAGE_BYTES;
+  const int q_s = p.ring_bytes;      // [8 rows][two steps][lane]: a thread's B fragments, 16 bytes
+  int* row_exp = reinterpret_cast<int*>(smem + q_s + rows_pad * DP * 2);
+  float* merged_ml = reinterpret_cast<float*>(row_exp + rows_pad);                  // [row][2]
   const int D = p.dim, qpk = p.heads / p.kv_heads;
+  const uint32_t bar0 = smem_u32(&bars[ring_no < WARPS ? ring_no : 0][0]);
+  const bool leads = !idle && warp == ring_no * p.row_groups * p.page_parts;      // its first lane asks for the first pages
+  if (leads && lane == 0) {
+    for (int st = 0; st < p.stages; ++st) {
+      mbar_init(bar0 + 8 * st, 1);
+      readers[ring_no][st] = 0;
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  pdl_entry();
 
   // this block's rows: row r of the block is head (row0 + r) % qpk of the group and token (row0 + r) / qpk of the tile
   int seq, q0 = 0, g, row0 = 0, tokens = 1;
@@ -143,41 +242,30 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) attention_q8_kernel(Ste
     tokens = min(p.tile_tokens, sb.seq_new[seq] - q0);
   }
   const int n_rows = min(rows_pad, tokens * qpk - row0);
-  if (n_rows <= 0) return;
+  if (n_rows <= 0) return;      // all blocks of a cluster alike
   const int past = sb.seq_past[seq], start = sb.seq_start[seq];
-  const int first_pos = past + q0 + row0 / qpk, last_pos = past + q0 + (row0 + n_rows - 1) / qpk;
+  const int first_pos = FUSED ? past : past + q0 + row0 / qpk, last_pos = FUSED ? past : past + q0 + (row0 + n_rows - 1) / qpk;
   const int low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;      // the first key that a row sees
   const int* pages = sb.pages + size_t(seq) * sb.pages_stride;
   const int split = blockIdx.z;
   // pages of this block (whole ones: the page that a step appends to has one reader), and of them this warp's tiles
   const int pg0 = low / PTB_PAGE, n_pages = last_pos / PTB_PAGE + 1 - pg0;
-  const int pg_begin = pg0 + int((long long)split * n_pages / p.n_splits), pg_end = pg0 + int((long long)(split + 1) * n_pages / p.n_splits);
-  const int t_begin = max(pg_begin * (PTB_PAGE / TILE), low / TILE), t_end = min(pg_end * (PTB_PAGE / TILE), last_pos / TILE + 1);
-
+  auto share = [&](int i) {
+    return n_pages < (1 << 21) ? i * n_pages / p.n_splits : int((long long)i * n_pages / p.n_splits);      // n_splits <= 512
+  };
+  const int pg_begin = pg0 + (p.n_splits == 1 ? 0 : share(split)), pg_end = pg0 + (p.n_splits == 1 ? n_pages : share(split + 1));
+  const bool appends = FUSED && p.write_cache && pg_end == pg0 + n_pages && pg_begin < pg_end;
   const int fused_width = p.kv_heads * (qpk + 2) * D;
-  if (FUSED && p.write_cache && pg_end == pg0 + n_pages && pg_begin < pg_end) {
-    const int page = pages[pg_end - 1];
-    const __nv_bfloat16* frow = p.rows + size_t(start) * fused_width + size_t(g) * (qpk + 2) * D;
-    if (page >= 0 && page < p.pool_pages) {
-      const size_t block = size_t(page) * p.kv_heads + g;
-      for (int which = warp; which < 2; which += nthreads >> 5) {
-        append_row(frow + size_t(qpk + which) * D, p.rope_cos + size_t(start) * p.rot_pairs, p.rope_sin + size_t(start) * p.rot_pairs,
-                   which == 0 ? p.rot_pairs : 0, p.interleaved, (which == 0 ? p.k_pool : p.v_pool) + block * PTB_PAGE * D,
-                   (which == 0 ? p.k_exp : p.v_exp) + block, past % PTB_PAGE, D);
-        __threadfence();
-      }
-    }
-    __syncthreads();
-  }
 
-  // what a lane knows of the warp's tile `lane` of a stretch of 32: its page and the page's exponents
-  const int n_mine = t_begin + kg < t_end && rg * 16 * MT < n_rows ? (t_end - t_begin - kg + p.key_groups - 1) / p.key_groups : 0;
+  const int n_mine = !idle && pg_begin + ring_no < pg_end && rg * 8 * NH < n_rows ? (pg_end - pg_begin - ring_no + p.rings - 1) / p.rings : 0;
+  const int sharers = p.page_parts * min(p.row_groups, (n_rows + 8 * NH - 1) / (8 * NH));      // warps that read a page of the ring
+  // what a lane knows of page `lane` of a stretch of 32 of the ring's: its number and its exponents
   auto look_up = [&](int stretch, int& page, int& exps) {
     const int i = stretch * 32 + lane;
     page = 0;
     exps = 0;
     if (i < n_mine) {
-      page = pages[(t_begin + kg + i * p.key_groups) / (PTB_PAGE / TILE)];
+      page = pages[pg_begin + ring_no + i * p.rings];
       if (page < 0 || page >= p.pool_pages) {
         atomicExch(p.error_flag, 21);
         page = 0;
@@ -187,323 +275,482 @@ __global__ void __launch_bounds__(256, DP == 64 ? 2 : 1) attention_q8_kernel(Ste
              (int(__ldcg(reinterpret_cast<const signed char*>(p.v_exp) + block)) & 255);
     }
   };
-  int spot[DP / 32];      // where this lane's 16-byte pieces of a tile go
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) {
-    const int piece = lane + 32 * i, per_row = D / 16;
-    spot[i] = piece < D ? place<DP>(piece / per_row, piece % per_row) : -1;
-  }
-  int page_now, exps_now, page_next = 0, exps_next = 0, exps_used;
+  int page_now, exps_now, page_next = 0, exps_next = 0;
   look_up(0, page_now, exps_now);
-  exps_used = exps_now;
-  auto issue = [&](int i) {
-    if (i < n_mine) {
-      if ((i & 31) == 0 && i > 0) {
-        page_now = page_next;
-        exps_now = exps_next;
-      }
-      if ((i & 31) == 16 && i + 16 < n_mine) look_up((i >> 5) + 1, page_next, exps_next);
-      const int page = __shfl_sync(0xffffffffu, page_now, i & 31);
-      const int t = t_begin + kg + i * p.key_groups;
-      const size_t from = ((size_t(page) * p.kv_heads + g) * PTB_PAGE + (t & 3) * TILE) * D + lane * 16;
-      const uint32_t to = smem_u32(ring + (i % STAGES) * Shape::STAGE_BYTES);
-#pragma unroll
-      for (int k = 0; k < DP / 32; ++k)
-        if (spot[k] >= 0) {
-          cp_async16(to + spot[k], p.k_pool + from + k * 512);
-          cp_async16(to + TILE * DP + spot[k], p.v_pool + from + k * 512);
-        }
-    }
-    copy_commit();
+  int page_ahead = page_now;      // of the stretch that pages are asked for from
+  auto page_of = [&](int i) {      // by every lane, for i one after another
+    if ((i & 31) == 0 && i > 0) page_ahead = page_next;
+    return __shfl_sync(0xffffffffu, page_ahead, i & 31);
   };
-  if (D < DP) {      // entries past the head size stay zero: no copy goes there
-    for (int i = lane; i < STAGES * Shape::STAGE_BYTES / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
-    __syncwarp();
+  auto ask = [&](int page, int st) {      // by one thread
+    const uint32_t bar = bar0 + 8 * st, to = smem_u32(smem) + ring + st * Shape::STAGE_BYTES;
+    const int y = (page * p.kv_heads + g) * PTB_PAGE;
+    mbar_expect_tx(bar, Shape::STAGE_BYTES);
+#pragma unroll
+    for (int x = 0; x < DP; x += 128) tma_load_2d(to + x * PTB_PAGE, &k_map, x, y, bar);
+#pragma unroll
+    for (int x = 0; x < DP; x += 128) tma_load_2d(to + PTB_PAGE * DP + x * PTB_PAGE, &v_map, x, y, bar);
+  };
+  auto ask_first = [&]() {
+    for (int st = 0; st < p.stages && st < n_mine; ++st) {
+      const int page = page_of(st);
+      if (lane == 0) ask(page, st);
+    }
+  };
+  if (leads) ask_first();      // on their way while the queries are made
+  if (appends) {
+    const int page = pages[pg_end - 1];
+    const __nv_bfloat16* frow = p.rows + size_t(start) * fused_width + size_t(g) * (qpk + 2) * D;
+    if (warp < 2) {
+      const int which = warp;
+      bool rose = false;
+      int e = 0;
+      if (page >= 0 && page < p.pool_pages) {
+        const size_t block = size_t(page) * p.kv_heads + g;
+        e = append_row(frow + size_t(qpk + which) * D, p.rope_cos + size_t(start) * p.rot_pairs, p.rope_sin + size_t(start) * p.rot_pairs,
+                       which == 0 ? p.rot_pairs : 0, p.interleaved, (which == 0 ? p.k_pool : p.v_pool) + block * PTB_PAGE * D,
+                       (which == 0 ? p.k_exp : p.v_exp) + block, past % PTB_PAGE, D, new_rows[which], rose);
+      }
+      if (lane == 0) {
+        new_exp[which] = e;
+        new_rose[which] = rose;
+      }
+    }
   }
-  for (int i = 0; i < STAGES - 1; ++i) issue(i);      // on their way while the queries are made
 
-  // queries: rotated (FUSED), brought to [1, 2) by a power of two, float16. A group of lanes holds a row, eight entries each.
+  // queries: rotated (FUSED), brought to [1, 2) by a power of two, float16. A group of lanes holds a row, eight entries each; the
+  // loads of four rows are out before the first is used.
   {
-    constexpr int GL = DP / 8, PER = 32 / GL;
-    const int c = lane % GL;
-    for (int r = warp * PER + lane / GL; r < rows_pad;      // rows_pad is a multiple of 16: a warp leaves as one
-         r += (nthreads >> 5) * PER) {
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (r < n_rows && c * 8 < D) {
-        if (FUSED) {
-          const __nv_bfloat16* row = p.rows + size_t(start) * fused_width + (size_t(g) * (qpk + 2) + r) * D;
-          load_rotated8(row, c, p.rope_cos + size_t(start) * p.rot_pairs, p.rope_sin + size_t(start) * p.rot_pairs, p.rot_pairs,
-                        p.interleaved, x);
-        } else {
-          const size_t t = start + q0 + (row0 + r) / qpk;
-          unpack_bf16x8(*reinterpret_cast<const uint4*>(p.rows + (t * p.heads + g * qpk + (row0 + r) % qpk) * D + c * 8), x);
+    constexpr int GL = DP / 8, PER = 32 / GL, AHEAD = 4;
+    const int c = lane % GL, step = WARPS * PER;
+    Angles angles;
+    angles.mode = 0;
+    angles.other = c;
+    const float *rc = p.rope_cos + size_t(start) * p.rot_pairs, *rs = p.rope_sin + size_t(start) * p.rot_pairs;
+    if (FUSED && c * 8 < D) angles = angles_of(c, rc, rs, p.rot_pairs, p.interleaved);
+    auto row_at = [&](int r) {
+      if (FUSED) return p.rows + size_t(start) * fused_width + (size_t(g) * (qpk + 2) + r) * D;
+      const size_t t = start + q0 + (row0 + r) / qpk;
+      return p.rows + (t * p.heads + g * qpk + (row0 + r) % qpk) * D;
+    };
+    for (int r0 = warp * PER + lane / GL; r0 < rows_pad; r0 += step * AHEAD) {
+      uint4 own[AHEAD], other[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = r0 + k * step;
+        own[k] = other[k] = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && c * 8 < D) {
+          const uint4* row = reinterpret_cast<const uint4*>(row_at(r));
+          own[k] = row[c];
+          if (FUSED && angles.mode == 2) other[k] = row[angles.other];
         }
       }
-      float most = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_abs(x[e]));
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = r0 + k * step;
+        if (r >= rows_pad) break;      // rows_pad and r0 - lane / GL are multiples of PER: a warp leaves as one
+        float x[8];
+        if (FUSED && angles.mode == 3 && r < n_rows) load_rotated8(row_at(r), c, rc, rs, p.rot_pairs, 0, x);
+        else rotate8(angles, own[k], other[k], x);
+        float most = 0.f;
 #pragma unroll
-      for (int o = GL / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const int e = min(max((__float_as_int(most) >> 23) - 127, -100), 126);      // most = 2^e * [1, 2)
-      const float by = power_of_two(-e);
-      uint4 w;
-      w.x = pack_half(x[0] * by, x[1] * by);
-      w.y = pack_half(x[2] * by, x[3] * by);
-      w.z = pack_half(x[4] * by, x[5] * by);
-      w.w = pack_half(x[6] * by, x[7] * by);
-      *reinterpret_cast<uint4*>(q_s + size_t(r) * Shape::Q_PITCH + c * 16) = w;
-      if (c == 0) row_exp[r] = e;
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_abs(x[e]));
+#pragma unroll
+        for (int o = GL / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int e = min(max((__float_as_int(most) >> 23) - 127, -100), 126);      // most = 2^e * [1, 2)
+        const float by = power_of_two(-e);
+        uint4 w;
+        w.x = pack_half(x[0] * by, x[1] * by);
+        w.y = pack_half(x[2] * by, x[3] * by);
+        w.z = pack_half(x[4] * by, x[5] * by);
+        w.w = pack_half(x[6] * by, x[7] * by);
+        // entries 8 c and on: two steps of the thread that holds this row and these 16 entries
+        *reinterpret_cast<uint4*>(smem + q_s + (((r >> 3) * (KS / 2) + (c >> 3) * 2 + (c & 1)) * 32 + (r & 7) * 4 + ((c >> 1) & 3)) * 16) = w;
+        if (c == 0) row_exp[r] = e;
+      }
     }
   }
   __syncthreads();
-
-  const float sl2 = p.scale * 1.4426950408889634f;
-  int row_pos[MT][2];
-  float row_fac[MT][2], slope[MT][2];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = (rg * MT + mt) * 16 + g4 + 8 * i;
-      const bool ok = r < n_rows;
-      row_pos[mt][i] = ok ? past + q0 + (row0 + r) / qpk : -1;
-      row_fac[mt][i] = power_of_two(row_exp[r]);
-      slope[mt][i] = ok && p.slopes ? p.slopes[g * qpk + (row0 + r) % qpk] : 0.f;
-      if (!p.slopes) row_fac[mt][i] *= sl2;
-    }
-  // A fragments of two k-steps from one 16-byte read a row
-  auto q_frags = [&](int mt, int step, uint32_t (&a)[4], uint32_t (&b)[4]) {      // steps `step` and step + 1
-    const unsigned char* at = q_s + size_t((rg * MT + mt) * 16 + g4) * Shape::Q_PITCH + ((step >> 2) * 64 + t4 * 16 + (step & 3) * 4) * 2;
-    const uint4 u = *reinterpret_cast<const uint4*>(at), d = *reinterpret_cast<const uint4*>(at + 8 * Shape::Q_PITCH);
-    a[0] = u.x; a[2] = u.y; b[0] = u.z; b[2] = u.w;
-    a[1] = d.x; a[3] = d.y; b[1] = d.z; b[3] = d.w;
+  // Waits are bounded: one that runs out raises the error flag, and the block goes on to its end.
+  bool alive = true;
+  int turn = 0;      // of the barriers: whether the first pages came twice
+  auto landed = [&](int i, int st, int parity) {
+    const uint32_t bar = bar0 + 8 * st;
+    if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 22));
   };
-  uint32_t qa[Q_REGS ? MT : 1][Q_REGS ? KS : 1][4];
-  if (Q_REGS) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int s = 0; s < KS; s += 2) q_frags(mt, s, qa[Q_REGS ? mt : 0][Q_REGS ? s : 0], qa[Q_REGS ? mt : 0][Q_REGS ? s + 1 : 0]);
+  if (appends) {
+    if (new_rose[0] || new_rose[1]) {      // the page's earlier codes have changed: the first pages once more
+      for (int st = 0; st < p.stages && st < n_mine && alive; ++st) landed(st, st, 0);
+      __syncthreads();
+      if (leads && alive) ask_first();
+      turn = 1;
+    }
+    if (lane < n_mine && pg_begin + ring_no + lane * p.rings == pg_end - 1) exps_now = new_exp[0] * 256 + (new_exp[1] & 255);
   }
 
-  float o[MT][NT][4];
+  const float sl2 = p.scale * 1.4426950408889634f;
+  float row_fac[NH][2];      // a thread's rows: 8 n + 2 t4 and the next, of its warp's
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NH; ++n)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
-  float m_run[MT][2], l_run[MT][2];
+    for (int i = 0; i < 2; ++i) {
+      row_fac[n][i] = power_of_two(row_exp[(rg * NH + n) * 8 + 2 * t4 + i]);
+      if (!p.slopes) row_fac[n][i] *= sl2;
+    }
+  const int q_at = q_s + rg * NH * (KS / 2) * 512 + lane * 16;
+  auto q_frag = [&](int n, int step) { return *reinterpret_cast<const uint4*>(smem + q_at + (n * (KS / 2) + step / 2) * 512); };      // of steps `step`, step + 1
+  uint4 qb[Q_REGS ? NH : 1][Q_REGS ? KS / 2 : 1];
+  if (Q_REGS) {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) m_run[mt][0] = m_run[mt][1] = -INFINITY, l_run[mt][0] = l_run[mt][1] = 0.f;
-  int unit = Q8_EXP_MIN, largest = Q8_EXP_MIN;      // of the output; of the values' exponents so far
+    for (int n = 0; n < NH; ++n)
+#pragma unroll
+      for (int s = 0; s < KS / 2; ++s) qb[Q_REGS ? n : 0][Q_REGS ? s : 0] = q_frag(n, 2 * s);
+  }
 
-  for (int i = 0; i < n_mine; ++i) {
-    copy_wait<STAGES - 2>();
-    __syncwarp();
-    issue(i + STAGES - 1);
-    if ((i & 31) == 0) exps_used = exps_now;      // the copies are fewer than 32 tiles ahead
-    const unsigned char* kt = ring + (i % STAGES) * Shape::STAGE_BYTES;
-    const unsigned char* vt = kt + TILE * DP;
-    const int key0 = (t_begin + kg + i * p.key_groups) * TILE;
-    const int both = __shfl_sync(0xffffffffu, exps_used, i & 31);
-    const int ev = int(int8_t(both & 255)), ek = (both - (both & 255)) >> 8;
+  float o[NH][KS][4];
+#pragma unroll
+  for (int n = 0; n < NH; ++n)
+#pragma unroll
+    for (int j = 0; j < KS; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+  float m_run[NH][2], l_run[NH][2];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) m_run[n][0] = m_run[n][1] = -INFINITY, l_run[n][0] = l_run[n][1] = 0.f;
+  int unit = Q8_EXP_MIN, largest = Q8_EXP_MIN;      // of the output; of the values' exponents so far
+  constexpr int VW = DP == 64 ? 2 : 4, VR = (DP + 127) / 128;      // words of a key's row a thread takes at a time, and times
+  // where in a stage a thread reads: its key of eight (the other eights 8 rows on, under the same swizzle), its keys of a value pair
+  int k_at[DP / 64], v_at[2];
+#pragma unroll
+  for (int r = 0; r < DP / 64; ++r) k_at[r] = ring + place<DP>(kappa<DP>(g4), t4 + 4 * r);
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    v_at[u] = ring + PTB_PAGE * DP + (DP == 64 ? place<DP>(kappa<DP>(2 * t4 + u), g4 >> 1) + (g4 & 1) * 8 : place<DP>(kappa<DP>(2 * t4 + u), g4));
+  constexpr int EIGHT = 8 * (DP == 64 ? 64 : 128);      // bytes from a row to that of eight keys on
+  const int part_keys = PTB_PAGE / p.page_parts;
+  int st = 0;
+
+  int i = 0;
+  for (; i < n_mine && alive; ++i) {
+    const int i_ahead = i + p.stages;
+    const int page_ahead_now = i_ahead < n_mine ? page_of(i_ahead) : 0;
+    if ((i & 31) == 0 && i > 0) exps_now = exps_next;
+    if ((i & 31) == 8 && (i & ~31) + 32 < n_mine) look_up((i >> 5) + 1, page_next, exps_next);
+    const int both = __shfl_sync(0xffffffffu, exps_now, i & 31);
+    const int page_key0 = (pg_begin + ring_no + i * p.rings) * PTB_PAGE;
+    landed(i, st, turn & 1);
+    if (!alive) break;
+    const int first_key = page_key0 + part * part_keys;
+    if (FUSED && appends && past - first_key >= 0 && past - first_key < part_keys) {
+      // the new token's codes from this block rather than from the page, where they may have come after the copy; all who read them
+      // write the same
+      if (lane < 2 * D / 16) {
+        const int which = lane >= D / 16, c = which ? lane - D / 16 : lane;
+        *reinterpret_cast<uint4*>(smem + ring + st * Shape::STAGE_BYTES + which * PTB_PAGE * DP + place<DP>(past - page_key0, c)) =
+            *reinterpret_cast<const uint4*>(new_rows[which] + c * 16);
+        proxy_fence_async();      // before the accelerator may write there again
+      }
+      __syncwarp();
+    }
+    const int ev = int(int8_t(both & 255)), ek = both >> 8;
+    for (int sub = 0; sub < part_keys; sub += TILE) {
+    const int key0 = first_key + sub;
+    if (key0 > last_pos || key0 + TILE <= low) continue;
+    const int kt = st * Shape::STAGE_BYTES + (key0 - page_key0) * (DP == 64 ? 64 : 128);
 
     // scores
-    float s[MT][2][4];
+    float s[NH][ST][4];      // of row 2 t4, 2 t4 + 1 with key kappa(g4), then with key 8 + kappa(g4)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
+      for (int j = 0; j < ST; ++j) s[n][j][0] = s[n][j][1] = s[n][j][2] = s[n][j][3] = 0.f;
 #pragma unroll
     for (int r = 0; r < DP / 64; ++r) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(kt + place<DP>(g4, t4 + 4 * r));
-      const uint4 k1 = *reinterpret_cast<const uint4*>(kt + place<DP>(8 + g4, t4 + 4 * r));
-      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+      uint4 w[2 * ST];
 #pragma unroll
-      for (int kk = 0; kk < 4; kk += 2) {
-        uint32_t b[2][2][2];
+      for (int j = 0; j < 2 * ST; ++j) w[j] = *reinterpret_cast<const uint4*>(smem + k_at[r] + kt + j * EIGHT);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          b[u][0][0] = q8_half2(w0[kk + u] & 0xffffu);
-          b[u][0][1] = q8_half2(w0[kk + u] >> 16);
-          b[u][1][0] = q8_half2(w1[kk + u] & 0xffffu);
-          b[u][1][1] = q8_half2(w1[kk + u] >> 16);
-        }
+      for (int kk = 0; kk < 4; ++kk) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t fa[4], fb[4];
-          if (!Q_REGS) q_frags(mt, r * 4 + kk, fa, fb);
-          const uint32_t(&a0)[4] = Q_REGS ? qa[Q_REGS ? mt : 0][Q_REGS ? r * 4 + kk : 0] : fa;
-          const uint32_t(&a1)[4] = Q_REGS ? qa[Q_REGS ? mt : 0][Q_REGS ? r * 4 + kk + 1 : 0] : fb;
-          mma_f16(s[mt][0], a0, b[0][0][0], b[0][0][1]);
-          mma_f16(s[mt][1], a0, b[0][1][0], b[0][1][1]);
-          mma_f16(s[mt][0], a1, b[1][0][0], b[1][0][1]);
-          mma_f16(s[mt][1], a1, b[1][1][0], b[1][1][1]);
+        for (int j = 0; j < ST; ++j) {
+          uint32_t a[4];
+          q8_halves(word_of(w[2 * j], kk), a[0], a[2]);
+          q8_halves(word_of(w[2 * j + 1], kk), a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            const uint4 q = Q_REGS ? qb[Q_REGS ? n : 0][Q_REGS ? r * 2 + kk / 2 : 0] : q_frag(n, r * 4 + kk);
+            mma_f16(s[n][j], a, (kk & 1) ? q.z : q.x, (kk & 1) ? q.w : q.y);
+          }
         }
       }
     }
-    // scale, bias and mask; a tile that all rows see whole needs no mask
-    const float fk = power_of_two(ek);
-    const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
-    bool moves = false;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int h = e >> 1;
-          float v = s[mt][j][e] * (row_fac[mt][h] * fk);
-          const int key = key0 + j * 8 + t4 * 2 + (e & 1);
-          if (p.slopes) v = (v + alibi_bias(slope[mt][h], key)) * sl2;
-          if (!whole && (key > row_pos[mt][h] || (p.window > 0 && key <= row_pos[mt][h] - p.window))) v = -INFINITY;
-          s[mt][j][e] = v;
-          moves = moves || v > m_run[mt][h] + MOVE_LOG2;
-        }
-    // the unit of the output, and the maxima where one has to move
+    // The unit of the output: that of the tile's values, but for a difference of 2^3 either way, which the weights carry instead (they
+    // stay within float16: 2^8 from the maximum that does not move, 2^3 from here), and for pages 2^60 below the largest.
     largest = max(largest, ev);
-    const int unit_new = max(ev, largest - UNIT_RANGE);
-    if (__any_sync(0xffffffffu, moves) || unit_new != unit) {
-      const float change = power_of_two(min(max(unit - unit_new, -126), 126));
+    const int floor_unit = largest - UNIT_RANGE;
+    const bool new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
+    const int old_unit = unit;
+    if (new_unit) unit = max(ev, floor_unit);
+    const int far = max(ev - unit, -126), shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
+    // score - running maximum + shift, in powers of two; a tile that all rows see whole needs no mask
+    const float fk = power_of_two(ek), fshift = float(shift);
+    const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
+    float over = -INFINITY;      // by how much the tile exceeds the running maxima
+    if (whole && !p.slopes) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float m = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          m = fmaxf(m, m_run[mt][h]);
-          const float corr = m_run[mt][h] == -INFINITY ? 0.f : exp2f(m_run[mt][h] - m);
-          m_run[mt][h] = m;
-          l_run[mt][h] *= corr;
+          const bool fresh = m_run[n][h] == -INFINITY;
+          const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < ST; ++j) {
+            s[n][j][h] = fmaf(s[n][j][h], f, m);
+            s[n][j][2 + h] = fmaf(s[n][j][2 + h], f, m);
+            top = fmaxf(top, fmaxf(s[n][j][h], s[n][j][2 + h]));
+          }
+          over = fmaxf(over, fresh ? INFINITY : top);
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = (rg * NH + n) * 8 + 2 * t4 + h;
+          const bool ok = r < n_rows;
+          const int pos = !ok ? -1 : FUSED ? past : past + q0 + (row0 + r) / qpk;
+          const float slope = ok && p.slopes ? p.slopes[g * qpk + (FUSED ? r : (row0 + r) % qpk)] : 0.f;
+          const bool fresh = m_run[n][h] == -INFINITY;
+          const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 2 * ST; ++j) {
+            const int key = key0 + j * 8 + kappa<DP>(g4);
+            float v = s[n][j >> 1][(j & 1) * 2 + h] * f;
+            if (p.slopes) v = (v + alibi_bias(slope, key)) * sl2;
+            v += m;
+            if (!whole && (key > pos || (p.window > 0 && key <= pos - p.window))) v = -INFINITY;
+            s[n][j >> 1][(j & 1) * 2 + h] = v;
+            top = fmaxf(top, v);
+          }
+          over = fmaxf(over, fresh && top != -INFINITY ? INFINITY : top);
+        }
+    }
+    if (__any_sync(0xffffffffu, over > MOVE_LOG2 + fshift) || new_unit) {
+      const float change = power_of_two(min(max(old_unit - unit, -126), 126));
+#pragma unroll
+      for (int n = 0; n < NH; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float up = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < ST; ++j) up = fmaxf(up, fmaxf(s[n][j][h], s[n][j][2 + h]));
+#pragma unroll
+          for (int lanes = 4; lanes < 32; lanes *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, lanes));
+          up -= fshift;
+          const bool fresh = m_run[n][h] == -INFINITY;      // then `up` is the maximum itself
+          if (!fresh) up = fmaxf(up, 0.f);
+          const float corr = fresh ? 0.f : exp2f(-up), by = up == -INFINITY ? 0.f : up;
+          m_run[n][h] = fresh ? up : m_run[n][h] + up;
+          l_run[n][h] *= corr;
+#pragma unroll
+          for (int j = 0; j < ST; ++j) {
+            s[n][j][h] -= by;
+            s[n][j][2 + h] -= by;
+          }
           const float f = corr * change;
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            o[mt][j][2 * h] *= f;
-            o[mt][j][2 * h + 1] *= f;
+          for (int j = 0; j < KS; ++j) {
+            o[n][j][h] *= f;
+            o[n][j][2 + h] *= f;
           }
         }
-      unit = unit_new;
     }
-    const float small = power_of_two(max(ev - unit, -126));      // 1 but for pages 2^60 below the largest
-    uint32_t pa[MT][4];
+    uint32_t pb[NH][ST][2];
+    const float back = power_of_two(-shift);      // the sums are of the weights themselves
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float w[2][4];
+    for (int n = 0; n < NH; ++n) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float m = m_run[mt][h] == -INFINITY ? 0.f : m_run[mt][h];
+      for (int j = 0; j < ST; ++j) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = fast_exp2(s[mt][j][2 * h + e] - m);
-            l_run[mt][h] += x;
-            w[j][2 * h + e] = x * small;
-          }
+        for (int e = 0; e < 4; ++e) s[n][j][e] = fast_exp2(s[n][j][e]);
+        l_run[n][0] = fmaf(s[n][j][0] + s[n][j][2], back, l_run[n][0]);
+        l_run[n][1] = fmaf(s[n][j][1] + s[n][j][3], back, l_run[n][1]);
       }
-      pa[mt][0] = pack_half(w[0][0], w[0][1]);
-      pa[mt][1] = pack_half(w[0][2], w[0][3]);
-      pa[mt][2] = pack_half(w[1][0], w[1][1]);
-      pa[mt][3] = pack_half(w[1][2], w[1][3]);
+      if (far != shift) {      // a page 2^60 below the largest: its weights are scaled before they are rounded
+#pragma unroll
+        for (int j = 0; j < ST; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][j][e] *= power_of_two(far);
+      }
+#pragma unroll
+      for (int j = 0; j < ST; ++j) {
+        pb[n][j][0] = transposed(pack_half(s[n][j][0], s[n][j][1]));
+        pb[n][j][1] = transposed(pack_half(s[n][j][2], s[n][j][3]));
+      }
     }
     // output. Keys that no row of the block sees are taken as zero: their codes may be anything.
     const bool edge = key0 + TILE - 1 > last_pos || key0 < low;
-    constexpr int VW = DP == 64 ? 2 : 4;      // words of a key's row a thread takes at a time
 #pragma unroll
-    for (int rr = 0; rr < (DP + 127) / 128; ++rr) {
-      uint32_t v[4][VW];
+    for (int ks = 0; ks < ST; ++ks)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int key = (u >> 1) * 8 + t4 * 2 + (u & 1);
-        if (DP == 64) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vt + place<DP>(key, g4 >> 1) + (g4 & 1) * 8);
-          v[u][0] = x.x; v[u][1] = x.y;
-        } else {
-          const uint4 x = *reinterpret_cast<const uint4*>(vt + place<DP>(key, g4 + 8 * rr));
-          v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
+      for (int rr = 0; rr < VR; ++rr) {
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int at = v_at[u & 1] + kt + rr * (PTB_PAGE * 128) + (2 * ks + (u >> 1)) * EIGHT;
+          if (DP == 64) {
+            const uint2 x = *reinterpret_cast<const uint2*>(smem + at);
+            v[u][0] = x.x; v[u][1] = x.y;
+          } else {
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + at);
+            v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
+          }
         }
-        if (edge && (key0 + key > last_pos || key0 + key < low)) {
+        if (edge) {
 #pragma unroll
-          for (int q = 0; q < VW; ++q) v[u][q] = 0u;
+          for (int u = 0; u < 4; ++u) {
+            const int key = key0 + (2 * ks + (u >> 1)) * 8 + kappa<DP>(2 * t4 + (u & 1));
+#pragma unroll
+            for (int q = 0; q < VW; ++q) v[u][q] = key > last_pos || key < low ? 0u : v[u][q];
+          }
         }
-      }
 #pragma unroll
-      for (int q = 0; q < VW; ++q) {
-        const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), a23 = __byte_perm(v[0][q], v[1][q], 0x7362);
-        const uint32_t c01 = __byte_perm(v[2][q], v[3][q], 0x5140), c23 = __byte_perm(v[2][q], v[3][q], 0x7362);
-        const uint32_t b0[4] = {q8_half2(a01 & 0xffffu), q8_half2(a01 >> 16), q8_half2(a23 & 0xffffu), q8_half2(a23 >> 16)};
-        const uint32_t b1[4] = {q8_half2(c01 & 0xffffu), q8_half2(c01 >> 16), q8_half2(c23 & 0xffffu), q8_half2(c23 >> 16)};
+        for (int q = 0; q < VW; ++q) {
+          uint32_t a[4], b[4];      // entries 4 q, 4 q + 1 and 4 q + 2, 4 q + 3 of the thread's
+          q8_halves(__byte_perm(v[0][q], v[1][q], 0x5140), a[0], a[1]);
+          q8_halves(__byte_perm(v[2][q], v[3][q], 0x5140), a[2], a[3]);
+          q8_halves(__byte_perm(v[0][q], v[1][q], 0x7362), b[0], b[1]);
+          q8_halves(__byte_perm(v[2][q], v[3][q], 0x7362), b[2], b[3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) mma_f16(o[mt][rr * 16 + q * 4 + e], pa[mt], b0[e], b1[e]);
+          for (int n = 0; n < NH; ++n) {
+            mma_f16(o[n][rr * 8 + q * 2], a, pb[n][ks][0], pb[n][ks][1]);
+            mma_f16(o[n][rr * 8 + q * 2 + 1], b, pb[n][ks][0], pb[n][ks][1]);
+          }
+        }
       }
     }
+    // the last warp to have read the page asks for the next one in its place
+    __syncwarp();
+    if (i_ahead < n_mine && lane == 0) {
+      __threadfence_block();
+      if (atomicAdd(&readers[ring_no][st], 1) == sharers - 1) {
+        readers[ring_no][st] = 0;
+        __threadfence_block();
+        ask(page_ahead_now, st);
+      }
+    }
+    if (++st == p.stages) st = 0, ++turn;
   }
-  copy_wait<0>();
-  __syncthreads();      // the rings are done with: the parts of the rows take their place
+  if (!alive)      // a wait ran out: what is in flight lands before the block ends (bounded waits again)
+    for (int k = 0; k < p.stages && i + k < n_mine; ++k) {
+      landed(i + k, st, turn & 1);
+      if (++st == p.stages) st = 0, ++turn;
+    }
 
-  // this warp's share of its rows: the mean of the values under its weights, in their own units, then maximum and sum
-  float* join = reinterpret_cast<float*>(rings);                                            // [key group][row][PITCH]
-  float* join_ml = join + size_t(p.key_groups) * rows_pad * Shape::PITCH;                   // [key group][row][2]
+  // Parts of a row into one, always in the same order: of the key groups here, of a cluster's blocks through their shared memory,
+  // of the teams of clusters by join_q8_kernel. Every part is a mean under its own weights times its share of the sum: the shares come
+  // before the sums of values, which may be as large as float32 holds.
+  float* join = reinterpret_cast<float*>(smem);                 // [key group][row][PITCH], in the rings' place
+  float* join_ml = merged_ml + 2 * rows_pad;                    // [key group][row][2]
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NH; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float l = l_run[mt][h];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      const int r = kg * rows_pad + (rg * MT + mt) * 16 + g4 + 8 * h;
-      const float inv = l == 0.f ? 0.f : power_of_two(unit) / l;
-      if (t4 == 0) {
-        join_ml[2 * r] = m_run[mt][h];
-        join_ml[2 * r + 1] = l;
+      float l = l_run[n][h];
+#pragma unroll
+      for (int lanes = 4; lanes < 32; lanes *= 2) l += __shfl_xor_sync(0xffffffffu, l, lanes);
+      l_run[n][h] = l;
+      const int r = kg * rows_pad + (rg * NH + n) * 8 + 2 * t4 + h;
+      if (g4 == 0 && !idle) *reinterpret_cast<float2*>(join_ml + 2 * r) = make_float2(m_run[n][h], l);
+    }
+  __syncthreads();      // and the rings are done with
+#pragma unroll
+  for (int n = 0; n < NH; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = (rg * NH + n) * 8 + 2 * t4 + h;
+      if (r >= n_rows || idle) continue;
+      float m = -INFINITY, l = 0.f;
+      for (int k = 0; k < key_groups; ++k) m = fmaxf(m, join_ml[2 * (k * rows_pad + r)]);
+      for (int k = 0; k < key_groups; ++k) {
+        const float2 ml = *reinterpret_cast<const float2*>(join_ml + 2 * (k * rows_pad + r));
+        l += ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.y * exp2f(ml.x - m);
       }
-      constexpr int COLS = DP == 64 ? 8 : 16;      // entries of the output in a row that a thread holds: [2 t4 + b][COLS]
-      float* to = join + size_t(r) * Shape::PITCH;
+      if (kg == 0 && g4 == 0) *reinterpret_cast<float2*>(merged_ml + 2 * r) = make_float2(m, l);
+      const bool none = m_run[n][h] == -INFINITY && l_run[n][h] == 0.f;
+      const float part = none ? 0.f : exp2f(m_run[n][h] - m) / l * power_of_two(unit);
+      constexpr int COLS = DP == 64 ? 8 : 16;      // entries of a row of the output that a thread holds: [g4][COLS]
+      float* to = join + size_t(kg * rows_pad + r) * Shape::PITCH + g4 * COLS;
 #pragma unroll
-      for (int rr = 0; rr < (DP + 127) / 128; ++rr)
+      for (int rr = 0; rr < VR; ++rr)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int c = 0; c < COLS; c += 4)
-            *reinterpret_cast<float4*>(to + rr * 128 + (2 * t4 + b) * COLS + c) =
-                make_float4(o[mt][rr * 16 + c][2 * h + b] * inv, o[mt][rr * 16 + c + 1][2 * h + b] * inv,
-                            o[mt][rr * 16 + c + 2][2 * h + b] * inv, o[mt][rr * 16 + c + 3][2 * h + b] * inv);
+        for (int c = 0; c < COLS / 2; c += 2) {
+          const float(&x)[4] = o[n][rr * 8 + c], (&y)[4] = o[n][rr * 8 + c + 1];
+          *reinterpret_cast<float4*>(to + rr * 128 + 2 * c) =
+              none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[h] * part, x[2 + h] * part, y[h] * part, y[2 + h] * part);
+        }
     }
   __syncthreads();
   const int quads = D / 4;
-  float* parts = p.n_splits > 1 ? p.parts + ((size_t(blockIdx.x) * gridDim.y + blockIdx.y) * p.n_splits + split) * size_t(rows_pad) * (D + 2) : nullptr;
-  for (int i = tid; i < n_rows * quads; i += nthreads) {
-    const int r = i / quads, d = (i - r * quads) * 4;
-    float m = -INFINITY;
-    for (int k = 0; k < p.key_groups; ++k) m = fmaxf(m, join_ml[2 * (k * rows_pad + r)]);
-    float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    auto weight = [&](int k) {
-      const float mk = join_ml[2 * (k * rows_pad + r)], lk = join_ml[2 * (k * rows_pad + r) + 1];
-      return mk == -INFINITY && lk == 0.f ? 0.f : lk * exp2f(mk - m);
-    };
-    for (int k = 0; k < p.key_groups; ++k) l += weight(k);      // always in this order
-    const float inv = l == 0.f ? 0.f : 1.f / l;      // before the values: they may be as large as float32 holds
-    for (int k = 0; k < p.key_groups; ++k) {
-      const float w = weight(k) * inv;
-      const float4 v = *reinterpret_cast<const float4*>(join + size_t(k * rows_pad + r) * Shape::PITCH + d);
-      if (w != 0.f) { acc[0] += v.x * w; acc[1] += v.y * w; acc[2] += v.z * w; acc[3] += v.w * w; }
-    }
-    if (p.n_splits > 1) {
-      float* to = parts + size_t(r) * (D + 2);
-      *reinterpret_cast<float2*>(to + d) = make_float2(acc[0], acc[1]);
-      *reinterpret_cast<float2*>(to + d + 2) = make_float2(acc[2], acc[3]);
+  auto write = [&](int r, int d, const float4& acc, float m, float l) {
+    if (p.teams > 1) {
+      float* to = p.parts + (((size_t(blockIdx.x) * gridDim.y + blockIdx.y) * p.teams + split / p.cluster) * rows_pad + r) * size_t(D + 2);
+      *reinterpret_cast<float2*>(to + d) = make_float2(acc.x, acc.y);
+      *reinterpret_cast<float2*>(to + d + 2) = make_float2(acc.z, acc.w);
       if (d == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, l);
     } else {
-      const size_t t = start + q0 + (row0 + r) / qpk;
-      *reinterpret_cast<uint2*>(p.out + (t * p.heads + g * qpk + (row0 + r) % qpk) * D + d) =
-          make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
+      const size_t t = start + q0 + (FUSED ? 0 : (row0 + r) / qpk);
+      *reinterpret_cast<uint2*>(p.out + (t * p.heads + g * qpk + (FUSED ? r : (row0 + r) % qpk)) * D + d) =
+          make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
     }
+  };
+  for (int i = tid; i < n_rows * quads; i += nthreads) {
+    const int r = i / quads, d = (i - r * quads) * 4;
+    float4 acc = *reinterpret_cast<const float4*>(join + size_t(r) * Shape::PITCH + d);
+    for (int k = 1; k < key_groups; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(join + size_t(k * rows_pad + r) * Shape::PITCH + d);
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    if (p.cluster > 1) *reinterpret_cast<float4*>(join + size_t(r) * Shape::PITCH + d) = acc;      // this thread alone reads and writes here
+    else write(r, d, acc, merged_ml[2 * r], merged_ml[2 * r + 1]);
   }
+  if (p.cluster == 1) return;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int n = p.cluster;
+  for (int i = tid * n + split % n; i < n_rows * quads; i += nthreads * n) {
+    const int r = i / quads, d = (i - r * quads) * 4;
+    float ms[MAX_CLUSTER], w[MAX_CLUSTER];
+    float4 v[MAX_CLUSTER];
+#pragma unroll
+    for (int k = 0; k < MAX_CLUSTER; ++k) {      // all on their way before the first is used
+      const int rank = k < n ? k : 0;
+      const float2 ml = *reinterpret_cast<const float2*>(cluster.map_shared_rank(merged_ml, rank) + 2 * r);
+      v[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(join, rank) + size_t(r) * Shape::PITCH + d);
+      ms[k] = k < n ? ml.x : -INFINITY;
+      w[k] = k < n ? ml.y : 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < MAX_CLUSTER; ++k) m = fmaxf(m, ms[k]);
+#pragma unroll
+    for (int k = 0; k < MAX_CLUSTER; ++k) {
+      w[k] = ms[k] == -INFINITY && w[k] == 0.f ? 0.f : w[k] * exp2f(ms[k] - m);
+      l += w[k];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < MAX_CLUSTER; ++k) {
+      const float u = w[k] * inv;
+      if (u != 0.f) { acc.x += v[k].x * u; acc.y += v[k].y * u; acc.z += v[k].z * u; acc.w += v[k].w * u; }
+    }
+    write(r, d, acc, m, l);
+  }
+  cluster.sync();      // no block leaves while another may still read its shared memory
 }
 
-// The splits' parts of a row into its output, always in the order of the splits.
+// The teams' parts of a row into its output, always in their order.
 template <bool FUSED>
 __global__ void __launch_bounds__(256) join_q8_kernel(StepBatch sb, AttnQ8 p, int rows_pad, int grid_y) {
   pdl_entry();
@@ -512,21 +759,21 @@ __global__ void __launch_bounds__(256) join_q8_kernel(StepBatch sb, AttnQ8 p, in
   const int seq = FUSED ? x : p.tile_seq[x], q0 = FUSED ? 0 : p.tile_q0[x];
   const int tokens = FUSED ? 1 : min(p.tile_tokens, sb.seq_new[seq] - q0);
   const int n_rows = min(rows_pad, tokens * qpk - row0), quads = D / 4;
-  const float* parts = p.parts + (size_t(x) * grid_y + y) * p.n_splits * size_t(rows_pad) * (D + 2);
+  const float* parts = p.parts + (size_t(x) * grid_y + y) * p.teams * size_t(rows_pad) * (D + 2);
   const size_t pitch = size_t(rows_pad) * (D + 2);
   for (int i = blockIdx.z * blockDim.x + threadIdx.x; i < n_rows * quads; i += gridDim.z * blockDim.x) {
     const int r = i / quads, d = (i - r * quads) * 4;
     const float* at = parts + size_t(r) * (D + 2);
     float m = -INFINITY;
-    for (int s = 0; s < p.n_splits; ++s) m = fmaxf(m, at[s * pitch + D]);
+    for (int s = 0; s < p.teams; ++s) m = fmaxf(m, at[s * pitch + D]);
     float l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     auto weight = [&](int s) {
       const float2 ml = *reinterpret_cast<const float2*>(at + s * pitch + D);
       return ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.y * exp2f(ml.x - m);
     };
-    for (int s = 0; s < p.n_splits; ++s) l += weight(s);
+    for (int s = 0; s < p.teams; ++s) l += weight(s);
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int s = 0; s < p.n_splits; ++s) {
+    for (int s = 0; s < p.teams; ++s) {
       const float w = weight(s) * inv;
       const float2 a = *reinterpret_cast<const float2*>(at + s * pitch + d), b = *reinterpret_cast<const float2*>(at + s * pitch + d + 2);
       if (w != 0.f) { acc[0] += a.x * w; acc[1] += a.y * w; acc[2] += b.x * w; acc[3] += b.y * w; }
@@ -538,32 +785,81 @@ __global__ void __launch_bounds__(256) join_q8_kernel(StepBatch sb, AttnQ8 p, in
 }
 
 struct Plan {
-  int dp, mt, row_groups, key_groups, rows_pad;
+  int dp, nh, row_groups, page_parts, rings, stages, rows_pad;
 };
 // rows: of a block's tile at most (more are divided among blocks)
-Plan plan_of(int dim, int rows) {
+Plan plan_of(int dim, int rows, bool fused) {
   Plan q;
   q.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  q.mt = rows > 16 && q.dp <= 128 ? 2 : 1;
-  const int groups = (rows + 16 * q.mt - 1) / (16 * q.mt), most = 8 / q.mt;
+  q.nh = rows <= 8 ? 1 : rows <= 16 || q.dp == 256 ? 2 : 4;
+  const int groups = (rows + 8 * q.nh - 1) / (8 * q.nh), most = q.dp == 256 ? 8 : q.dp == 128 && !fused ? 2 : 4;
   q.row_groups = groups < most ? groups : most;
-  q.key_groups = 8 / q.row_groups;
-  q.rows_pad = q.row_groups * 16 * q.mt;
+  q.rows_pad = q.row_groups * 8 * q.nh;
+  const int keys = WARPS / q.row_groups, parts = q.dp == 64 ? 2 : 4;      // a part is a tile at least
+  q.page_parts = keys >= parts ? parts : keys >= 2 ? 2 : 1;
+  q.rings = keys / q.page_parts;
+  // about 96 KB of rings where two blocks are to fit on an SM, else 128
+  const int pages = (q.nh == 4 || q.dp == 256 ? 131072 : 98304) / (2 * PTB_PAGE * q.dp);
+  q.stages = pages / q.rings < MAX_STAGES ? pages / q.rings : MAX_STAGES;
   return q;
 }
 
-template <int DP, int MT, bool FUSED>
-int launch_attn(const StepBatch& sb, const AttnQ8& p, const Plan& q, dim3 grid, cudaStream_t stream) {
-  using Shape = Q8Shape<DP>;
-  const int warps = q.row_groups * q.key_groups;
-  const size_t ring = size_t(warps) * Shape::STAGES * Shape::STAGE_BYTES;
-  const size_t join = size_t(q.key_groups) * q.rows_pad * (Shape::PITCH + 2) * sizeof(float);
-  const size_t smem = size_t(q.rows_pad) * (Shape::Q_PITCH + sizeof(int)) + (ring > join ? ring : join);
+// The codes of a pool as rows of `dim` bytes: boxes of a page's rows, 64 bytes or 128 wide (zeros past dim), under the swizzle of that width.
+bool codes_map(CUtensorMap* map, const void* pool, int pool_pages, int kv_heads, int dim, int dp) {
+  static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+  PFN_cuTensorMapEncodeTiled_v12000 encode = known.load(std::memory_order_acquire);
+  if (encode == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) != cudaSuccess || qr != cudaDriverEntryPointSuccess)
+      return false;
+    encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    known.store(encode, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {cuuint64_t(dim), cuuint64_t(pool_pages) * kv_heads * PTB_PAGE};
+  const cuuint64_t strides[1] = {cuuint64_t(dim)};
+  const cuuint32_t box[2] = {dp == 64 ? 64u : 128u, cuuint32_t(PTB_PAGE)};
+  const cuuint32_t elem[2] = {1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                dp == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, int NH, bool FUSED>
+int launch_attn(const StepBatch& sb, AttnQ8 p, const Plan& q, dim3 grid, cudaStream_t stream) {
+  using Shape = Q8Shape<DP, NH>;
+  const int key_groups = q.page_parts * q.rings;
+  const size_t ring = size_t(q.rings) * q.stages * Shape::STAGE_BYTES;
+  const size_t join = size_t(key_groups) * q.rows_pad * Shape::PITCH * sizeof(float);
+  p.ring_bytes = int(ring > join ? ring : (join + 15) / 16 * 16);
+  const size_t smem = 1024 + p.ring_bytes + size_t(q.rows_pad) * (DP * 2 + sizeof(int) + 2 * sizeof(float) * (1 + key_groups));
   static SharedLimit limit;
-  if (!limit.allows(attention_q8_kernel<DP, MT, FUSED>, smem)) return PTB_ERR_LAUNCH;
-  launch_pdl(attention_q8_kernel<DP, MT, FUSED>, grid, dim3(warps * 32), smem, stream, sb, p);
+  if (!limit.allows(attention_q8_kernel<DP, NH, FUSED>, smem)) return PTB_ERR_LAUNCH;
+  CUtensorMap k_map, v_map;
+  if (!codes_map(&k_map, p.k_pool, p.pool_pages, p.kv_heads, p.dim, DP) ||
+      !codes_map(&v_map, p.v_pool, p.pool_pages, p.kv_heads, p.dim, DP))
+    return PTB_ERR_LAUNCH;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  bool captured = true;      // launch_pdl's rule
+  if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess) captured = capture != cudaStreamCaptureStatusNone;
+  else (void)cudaGetLastError();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = captured ? 0 : 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = unsigned(p.cluster);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = captured ? attr + 1 : attr;
+  cfg.numAttrs = (captured ? 0 : 1) + (p.cluster > 1 ? 1 : 0);
+  cudaLaunchKernelEx(&cfg, attention_q8_kernel<DP, NH, FUSED>, sb, p, k_map, v_map);
   int status = launch_status();
-  if (status == PTB_OK && p.n_splits > 1) {
+  if (status == PTB_OK && p.teams > 1) {
     const int z = max(1, min(8, q.rows_pad * (p.dim / 4) / 512));
     launch_pdl(join_q8_kernel<FUSED>, dim3(grid.x, grid.y, z), dim3(256), 0, stream, sb, p, q.rows_pad, int(grid.y));
     status = launch_status();
@@ -572,32 +868,52 @@ int launch_attn(const StepBatch& sb, const AttnQ8& p, const Plan& q, dim3 grid, 
 }
 template <bool FUSED>
 int launch_any(const StepBatch& sb, const AttnQ8& p, const Plan& q, dim3 grid, cudaStream_t stream) {
-  if (q.dp == 64) return q.mt == 1 ? launch_attn<64, 1, FUSED>(sb, p, q, grid, stream) : launch_attn<64, 2, FUSED>(sb, p, q, grid, stream);
-  if (q.dp == 128) return q.mt == 1 ? launch_attn<128, 1, FUSED>(sb, p, q, grid, stream) : launch_attn<128, 2, FUSED>(sb, p, q, grid, stream);
-  return launch_attn<256, 1, FUSED>(sb, p, q, grid, stream);
+#define PTB_Q8(DD, NN) return launch_attn<DD, NN, FUSED>(sb, p, q, grid, stream)
+  if (q.dp == 64) {
+    if (q.nh == 1) PTB_Q8(64, 1);
+    if (q.nh == 2) PTB_Q8(64, 2);
+    PTB_Q8(64, 4);
+  }
+  if (q.dp == 128) {
+    if (q.nh == 1) PTB_Q8(128, 1);
+    if (q.nh == 2) PTB_Q8(128, 2);
+    PTB_Q8(128, 4);
+  }
+  if (q.nh == 1) PTB_Q8(256, 1);
+  PTB_Q8(256, 2);
+#undef PTB_Q8
 }
 bool known(int heads, int kv_heads, int dim, int pool_pages) {
-  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && dim >= 16 && dim <= 256 && dim % 16 == 0 && pool_pages > 0;
+  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && dim >= 16 && dim <= 256 && dim % 16 == 0 && pool_pages > 0 &&
+         (long long)pool_pages * kv_heads * PTB_PAGE < (1ll << 31);      // rows of codes, as the copies count them
 }
-// Blocks that share a row's pages: about two on every SM in all (one where a block's rings take its shared memory), each with four pages.
-int splits_of(long long blocks, int pages, int dp) {
-  const long long want = (dp == 64 ? 2ll : 1ll) * sm_count() / (blocks > 0 ? blocks : 1);
-  const long long most = pages / 4 < 64 ? pages / 4 : 64;
-  return int(want < 1 || most < 1 ? 1 : want < most ? want : most);
+// Blocks that share a row's pages: about two waves of them on the SMs in all, each with four pages at least. Up to eight form a cluster
+// and join through its shared memory; more are a multiple of eight, whose clusters join through a workspace.
+int splits_of(long long blocks, int pages, int dp, int nh) {
+  const long long slots = (nh == 4 || dp == 256 ? 1ll : 2ll) * sm_count();
+  long long want = (2 * slots + blocks - 1) / (blocks > 0 ? blocks : 1);
+  if (blocks >= 8 * slots) want = 1;
+  const long long most = pages / 4;
+  if (want > most) want = most;
+  if (want > MAX_CLUSTER) want = want / MAX_CLUSTER * MAX_CLUSTER;
+  return int(want < 1 ? 1 : want > 512 ? 512 : want);
 }
+int teams_of(int n_splits) { return n_splits <= MAX_CLUSTER ? 1 : n_splits / MAX_CLUSTER; }
+bool splits_known(int n_splits) { return n_splits >= 1 && n_splits <= 512 && (n_splits <= MAX_CLUSTER || n_splits % MAX_CLUSTER == 0); }
 }  // namespace
 
-// How many blocks share a row's pages (n_splits below) and the floats of workspace that they need: rows = query heads of a K/V head times
+// How many blocks share a row's pages (n_splits below: 1 to 8, or a multiple of 8) and the floats of workspace that they need: rows = query heads of a K/V head times
 // tokens of a tile; tiles = sequences of a step of single tokens, or tiles of a prompt; pages: that a row may see, at most.
-PTB_API int ptb_attention_q8_splits(int tiles, int kv_heads, int rows, int dim, int pages) {
-  const Plan q = plan_of(dim, rows);
+PTB_API int ptb_attention_q8_splits(int tiles, int kv_heads, int rows, int dim, int pages, int fused) {
+  const Plan q = plan_of(dim, rows, fused != 0);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
-  return splits_of((long long)tiles * kv_heads * chunks, pages, q.dp);
+  return splits_of((long long)tiles * kv_heads * chunks, pages, q.dp, q.nh);
 }
-PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int dim, int n_splits) {
-  const Plan q = plan_of(dim, rows);
+PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int dim, int n_splits, int fused) {
+  const Plan q = plan_of(dim, rows, fused != 0);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
-  return n_splits > 1 ? (long long)tiles * kv_heads * chunks * n_splits * q.rows_pad * (dim + 2) : 0;
+  const int teams = teams_of(n_splits);
+  return teams > 1 ? (long long)tiles * kv_heads * chunks * teams * q.rows_pad * (dim + 2) : 0;
 }
 
 // A step of single tokens. fused [n_seqs, kv_heads * (heads / kv_heads + 2) * dim] bfloat16, out [n_seqs, heads * dim]; pools and exponents as
@@ -608,17 +924,18 @@ PTB_API int ptb_attention_decode_q8(const void* fused, void* k_pool, void* k_exp
                                     int n_splits, float* parts, long long part_floats, int* error_flag, cudaStream_t stream) {
   if (sb->n_seqs <= 0) return PTB_OK;
   if (!known(heads, kv_heads, dim, pool_pages) || heads / kv_heads > 128 || sb->n_tokens != sb->n_seqs || rot_pairs < 0 || 2 * rot_pairs > dim ||
-      window < 0 || n_splits < 1 || n_splits > 65535 || error_flag == nullptr || (rot_pairs > 0 && (rope_cos == nullptr || rope_sin == nullptr)))
+      window < 0 || !splits_known(n_splits) || error_flag == nullptr || (rot_pairs > 0 && (rope_cos == nullptr || rope_sin == nullptr)))
     return PTB_ERR_SIZE;
   if (!aligned16(fused) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
-  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, heads / kv_heads, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
+  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, heads / kv_heads, dim, n_splits, 1) > part_floats) return PTB_ERR_SIZE;
   AttnQ8 p = {};
   p.rows = (const __nv_bfloat16*)fused; p.k_pool = (uint8_t*)k_pool; p.v_pool = (uint8_t*)v_pool; p.k_exp = (int8_t*)k_exp;
   p.v_exp = (int8_t*)v_exp; p.out = (__nv_bfloat16*)out; p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.slopes = slopes;
   p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pool_pages = pool_pages; p.rot_pairs = rot_pairs; p.interleaved = interleaved;
   p.write_cache = write_cache; p.window = window; p.n_splits = n_splits; p.scale = scale; p.parts = parts; p.error_flag = error_flag;
-  const Plan q = plan_of(dim, heads / kv_heads);
-  p.row_groups = q.row_groups; p.key_groups = q.key_groups;
+  const Plan q = plan_of(dim, heads / kv_heads, true);
+  p.row_groups = q.row_groups; p.page_parts = q.page_parts; p.rings = q.rings; p.stages = q.stages;
+  p.teams = teams_of(n_splits); p.cluster = n_splits / p.teams;
   return launch_any<true>(*sb, p, q, dim3(sb->n_seqs, kv_heads, n_splits), stream);
 }
 
@@ -629,13 +946,13 @@ PTB_API int ptb_attention_q8(const void* q_rows, const void* k_pool, const void*
                              const float* slopes, int heads, int kv_heads, int dim, float scale, int window, int n_splits, float* parts,
                              long long part_floats, int* error_flag, cudaStream_t stream) {
   if (n_tiles <= 0) return PTB_OK;
-  if (!known(heads, kv_heads, dim, pool_pages) || window < 0 || n_splits < 1 || n_splits > 65535 || error_flag == nullptr || tile_tokens < 1 ||
+  if (!known(heads, kv_heads, dim, pool_pages) || window < 0 || !splits_known(n_splits) || error_flag == nullptr || tile_tokens < 1 ||
       (long long)tile_tokens * (heads / kv_heads) > (1 << 24))
     return PTB_ERR_SIZE;
   if (!aligned16(q_rows) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
   const int rows = tile_tokens * (heads / kv_heads);
-  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
-  const Plan q = plan_of(dim, rows);
+  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, dim, n_splits, 0) > part_floats) return PTB_ERR_SIZE;
+  const Plan q = plan_of(dim, rows, false);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
   if (chunks * kv_heads > 65535) return PTB_ERR_SIZE;
   AttnQ8 p = {};
@@ -643,6 +960,7 @@ PTB_API int ptb_attention_q8(const void* q_rows, const void* k_pool, const void*
   p.v_exp = (int8_t*)v_exp; p.out = (__nv_bfloat16*)out; p.slopes = slopes; p.tile_seq = tile_seq; p.tile_q0 = tile_q0;
   p.tile_tokens = tile_tokens; p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pool_pages = pool_pages; p.window = window;
   p.n_splits = n_splits; p.scale = scale; p.parts = parts; p.error_flag = error_flag;
-  p.row_groups = q.row_groups; p.key_groups = q.key_groups;
+  p.row_groups = q.row_groups; p.page_parts = q.page_parts; p.rings = q.rings; p.stages = q.stages;
+  p.teams = teams_of(n_splits); p.cluster = n_splits / p.teams;
   return launch_any<false>(*sb, p, q, dim3(n_tiles, unsigned(chunks * kv_heads), n_splits), stream);
 }

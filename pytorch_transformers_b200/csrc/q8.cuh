@@ -31,14 +31,13 @@ __device__ __forceinline__ uint32_t q8_pack4(float a, float b, float c, float d)
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(d), "f"(c));
   return uint32_t(lo) | (uint32_t(hi) << 16);
 }
-// two codes as a pair of float16 numbers, exactly (the first in the lower half)
-__device__ __forceinline__ uint32_t q8_half2(uint32_t two) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;\n" : "=r"(h) : "h"(uint16_t(two)));
-  return h;
+// four codes as two pairs of float16 numbers, exactly (the first in the lower half)
+__device__ __forceinline__ void q8_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}\n" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ void q8_unpack4(uint32_t w, float (&f)[4]) {
-  const uint32_t lo = q8_half2(w & 0xffffu), hi = q8_half2(w >> 16);
+  uint32_t lo, hi;
+  q8_halves(w, lo, hi);
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}\n" : "=f"(f[0]), "=f"(f[1]) : "r"(lo));
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}\n" : "=f"(f[2]), "=f"(f[3]) : "r"(hi));
 }

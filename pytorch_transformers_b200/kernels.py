@@ -127,6 +127,15 @@ def lib():
         L.ptb_expert_plan_words.restype = ctypes.c_longlong
         L.ptb_mlstm_chunks_scratch_floats.restype = ctypes.c_longlong
         L.ptb_attention_q8_floats.restype = ctypes.c_longlong
+        # declared arguments: addresses and numbers go in as Python's own, which an eager call of a few microseconds notices
+        P, I, N, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+        L.ptb_store_q8.argtypes = [P] * 6 + [I, P, P, P] + [I] * 5 + [P, P]
+        L.ptb_unpack_q8.argtypes = [P] * 4 + [I, P, P, P, I, I, P, P, I, I, I, P, P]
+        L.ptb_attention_q8_splits.argtypes = [I] * 6
+        L.ptb_attention_q8_floats.argtypes = [I] * 6
+        L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, P, N, P, P]
+        L.ptb_attention_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, P, N, P, P]
+        L.ptb_copy_pages.argtypes = [P] * 6 + [I, P, P, N, I, I, P]
         _configured = True
     return L
 
@@ -505,10 +514,13 @@ def _with_index(device) -> torch.device:
 
 def error_flag(device) -> torch.Tensor:
     """Device int32 word that kernels with bounded waits raise when a wait runs out."""
-    device = _with_index(device)
-    if device not in _error_flags:
-        _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    return _error_flags[device]
+    flag = _error_flags.get(device)
+    if flag is None:
+        device = _with_index(device)
+        flag = _error_flags.get(device)
+        if flag is None:
+            flag = _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
+    return flag
 
 
 def check_device_errors(device) -> None:
@@ -1794,9 +1806,12 @@ def q8_supports(head_dim: int) -> bool:
     return 16 <= head_dim <= 256 and head_dim % 16 == 0
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
 def _on_device(t: torch.Tensor):
     """The device guard of ``t``'s device where it is not the current one (a launch goes to a stream of the current device)."""
-    return contextlib.nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _NO_GUARD if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Tensor, seq_new: torch.Tensor, seq_past: torch.Tensor,
@@ -1805,50 +1820,55 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
     sequence and position of every token, each sequence's first token, tokens of this step and tokens before it, and the page
     table [sequences, width]. The tensors must outlive the kernels that read them."""
     for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages):
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+        if not (t.dtype is torch.int32 and t.is_cuda and t.is_contiguous()):
             raise KernelError("step_batch takes contiguous int32 tensors on the device")
-    n = seq_start.numel()
-    if tok_seq.numel() != tok_pos.numel() or seq_new.numel() != n or seq_past.numel() != n or pages.dim() != 2 or pages.shape[0] != n:
+    n, tokens, table = seq_start.numel(), tok_seq.numel(), pages.shape
+    if tok_pos.numel() != tokens or seq_new.numel() != n or seq_past.numel() != n or len(table) != 2 or table[0] != n:
         raise KernelError("step_batch: the arrays' lengths do not fit one another")
     return StepBatchC(tok_seq.data_ptr(), tok_pos.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), seq_past.data_ptr(),
-                      pages.data_ptr(), pages.shape[1], tok_seq.numel(), n)
+                      pages.data_ptr(), table[1], tokens, n)
 
 
-def _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads: int, head_dim: int, device, what: str) -> None:
-    for pool, exp in ((k_pool, k_exp), (v_pool, v_exp)):
-        if (pool.dtype != Q8 or exp.dtype != torch.int8 or pool.dim() != 4 or pool.shape[1:] != (kv_heads, PAGE, head_dim)
-                or exp.shape != pool.shape[:2] or not pool.is_contiguous() or not exp.is_contiguous()
-                or pool.device != device or exp.device != device):
-            raise KernelError(f"{what} takes e4m3 pages [pages, {kv_heads}, {PAGE}, {head_dim}] and their int8 exponents [pages, "
-                              f"{kv_heads}], contiguous, on the device of the other tensors")
-    if k_pool.shape[0] != v_pool.shape[0]:
-        raise KernelError(f"{what}: keys and values have {k_pool.shape[0]} and {v_pool.shape[0]} pages")
+def _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads: int, head_dim: int, device: int, what: str) -> int:
+    """The pages of a cache entry in 8 bits, after a look at its tensors (``device``: the number of the others')."""
+    shape = k_pool.shape
+    if not (k_pool.dtype is Q8 and v_pool.dtype is Q8 and k_exp.dtype is torch.int8 and v_exp.dtype is torch.int8
+            and shape[1:] == (kv_heads, PAGE, head_dim) and v_pool.shape == shape and k_exp.shape == v_exp.shape == shape[:2]
+            and k_pool.is_contiguous() and v_pool.is_contiguous() and k_exp.is_contiguous() and v_exp.is_contiguous()
+            and k_pool.get_device() == v_pool.get_device() == k_exp.get_device() == v_exp.get_device() == device >= 0):
+        raise KernelError(f"{what} takes e4m3 pages [pages, {kv_heads}, {PAGE}, {head_dim}] and their int8 exponents [pages, "
+                          f"{kv_heads}], as many for keys as for values, contiguous, on the device of the other tensors")
     if not q8_supports(head_dim):
         raise KernelError(f"{what} takes head sizes that are multiples of 16 up to 256, got {head_dim}")
+    return shape[0]
 
 
-def _check_fused_q8(fused, batch, rope, kv_heads: int, q_per_kv: int, head_dim: int, what: str) -> int:
-    """The pairs that ``rope`` rotates, after a look at what the kernels take for granted."""
-    if not fused.is_cuda or fused.dtype != torch.bfloat16 or not fused.is_contiguous():
+def _check_fused_q8(fused, batch, rope, kv_heads: int, q_per_kv: int, head_dim: int, what: str):
+    """Addresses of cosines and sines and the pairs that they rotate, after a look at what the kernels take for granted."""
+    if not (fused.is_cuda and fused.dtype is torch.bfloat16 and fused.is_contiguous()):
         raise KernelError(f"{what} takes a contiguous bfloat16 projection on a CUDA device")
     n = batch.n_tokens
-    if tuple(fused.shape) != (n, kv_heads * (q_per_kv + 2) * head_dim):
+    if fused.shape != (n, kv_heads * (q_per_kv + 2) * head_dim):
         raise KernelError(f"{what}: the projection has shape {tuple(fused.shape)}, expected "
                           f"{(n, kv_heads * (q_per_kv + 2) * head_dim)}")
     if rope is None:
-        return 0
-    for t in rope:
-        if t.dtype != torch.float32 or t.device != fused.device or not t.is_contiguous() or t.dim() != 2 or t.shape[0] != n:
-            raise KernelError(f"{what}: cosines and sines must be contiguous float32 tensors [tokens, pairs] on the projection's device")
-    if rope[0].shape != rope[1].shape or 2 * rope[0].shape[1] > head_dim:
-        raise KernelError(f"{what}: {rope[0].shape[1]} and {rope[1].shape[1]} pairs do not fit a head of {head_dim}")
-    return rope[0].shape[1]
+        return None, None, 0
+    cos, sin = rope
+    shape = cos.shape
+    if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.is_contiguous() and sin.is_contiguous() and len(shape) == 2
+            and shape[0] == n and sin.shape == shape and cos.get_device() == sin.get_device() == fused.get_device()):
+        raise KernelError(f"{what}: cosines and sines must be contiguous float32 tensors [tokens, pairs] on the projection's device")
+    if 2 * shape[1] > head_dim:
+        raise KernelError(f"{what}: {shape[1]} pairs do not fit a head of {head_dim}")
+    return cos.data_ptr(), sin.data_ptr(), shape[1]
 
 
-def _check_slopes(slopes, heads: int, device, what: str) -> None:
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.numel() != heads or slopes.device != device
-                               or not slopes.is_contiguous()):
+def _check_slopes(slopes, heads: int, device: int, what: str):
+    if slopes is None:
+        return None
+    if not (slopes.dtype is torch.float32 and slopes.numel() == heads and slopes.get_device() == device and slopes.is_contiguous()):
         raise KernelError(f"{what}: slopes must be {heads} contiguous float32 numbers on the device of the other tensors")
+    return slopes.data_ptr()
 
 
 def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
@@ -1859,36 +1879,30 @@ def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torc
     e with max |x| <= 448 * 2^e); one with earlier tokens keeps its own unless the rows need a larger one, to which the earlier
     codes are then rounded again. What is infinite or no number is held as no number. bfloat16."""
     what = "split_rotate_store_q8"
-    pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
-    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.device, what)
-    cos, sin = rope if rope is not None else (None, None)
-    q = torch.empty((fused.shape[0], kv_heads * q_per_kv, head_dim), dtype=fused.dtype, device=fused.device)
+    cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
+    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.get_device(), what)
+    q = fused.new_empty((fused.shape[0], kv_heads * q_per_kv, head_dim))
+    cache = (k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr()) if write_cache else (None,) * 4
     with _on_device(fused):
-        _check(lib().ptb_store_q8(_ptr(fused), _ptr(q), *((_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp)) if write_cache
-                                                          else (None, None, None, None)), k_pool.shape[0], ctypes.byref(batch),
-                                  _ptr(cos), _ptr(sin), pairs, 1 if interleaved else 0, kv_heads, q_per_kv, head_dim,
-                                  _ptr(error_flag(fused.device)), _stream(fused)), what)
+        _check(lib().ptb_store_q8(fused.data_ptr(), q.data_ptr(), *cache, pages, ctypes.byref(batch), cos, sin, pairs, interleaved,
+                                  kv_heads, q_per_kv, head_dim, error_flag(fused.device).data_ptr(), _stream(fused)), what)
     return q
 
 
 def unpack_pages_q8(k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor, ids: torch.Tensor):
     """The pages that ``ids`` (int32, on the device) names as bfloat16 values, keys and values: [len(ids), kv_heads, PAGE, head_dim]
     each. A page out of range reads as zeros and raises the device's error flag."""
-    if ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous() or not ids.is_cuda or k_pool.dim() != 4:
+    if not (ids.dtype is torch.int32 and ids.dim() == 1 and ids.is_contiguous() and ids.is_cuda and k_pool.dim() == 4):
         raise KernelError("unpack_pages_q8 takes pages of one cache entry and a contiguous int32 list of page numbers on the device")
-    kv_heads, head_dim = k_pool.shape[1], k_pool.shape[3]
-    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, ids.device, "unpack_pages_q8")
-    out = torch.empty((2, ids.numel(), kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device)
+    _, kv_heads, _, head_dim = k_pool.shape
+    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, ids.get_device(), "unpack_pages_q8")
+    n = ids.numel()
+    k, v = torch.empty((2, n, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device).unbind(0)
     with _on_device(ids):
-        _check(lib().ptb_unpack_q8(_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(ids), None, None,
-                                   ids.numel(), 0, _ptr(out[0]), _ptr(out[1]), kv_heads, head_dim, head_dim,
-                                   _ptr(error_flag(ids.device)), _stream(ids)), "unpack_pages_q8")
-    return out[0], out[1]
-
-
-def _q8_parts(L, tiles: int, kv_heads: int, rows: int, head_dim: int, n_splits: int, device):
-    floats = L.ptb_attention_q8_floats(tiles, kv_heads, rows, head_dim, n_splits) if n_splits > 1 else 0
-    return (torch.empty(floats, dtype=torch.float32, device=device) if floats else None), floats
+        _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pages, ids.data_ptr(), None,
+                                   None, n, 0, k.data_ptr(), v.data_ptr(), kv_heads, head_dim, head_dim,
+                                   error_flag(ids.device).data_ptr(), _stream(ids)), "unpack_pages_q8")
+    return k, v
 
 
 def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
@@ -1896,67 +1910,84 @@ def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.
                         scale: float, window: int = 0, write_cache: bool = True, interleaved: bool = False, n_splits: int = 0,
                         max_pages: int = 0) -> torch.Tensor:
     """The attention of a step of single tokens over a cache in 8 bits: rotate the tokens' queries and keys, append key and value
-    to their pages (as ``split_rotate_store_q8`` does), attend. ``n_splits`` blocks share a sequence's pages (0: chosen from the
-    sizes and ``max_pages``, the most pages that a sequence of the step spans; by default the page table's width). At most 128
-    query heads a K/V head; head sizes are multiples of 16 up to 256. Returns [tokens, heads * head_dim]."""
+    to their pages (as ``split_rotate_store_q8`` does), attend. ``n_splits`` blocks share a sequence's pages (more than eight
+    in multiples of eight; 0: chosen from the sizes and ``max_pages``, the most pages that a sequence of the step spans, by default the
+    page table's width). At most 128 query heads a K/V head; head sizes are multiples of 16 up to 256. Returns [tokens, heads * head_dim]."""
     what = "attention_decode_q8"
-    pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
-    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.device, what)
+    cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
+    device = fused.get_device()
+    pool_pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     heads = kv_heads * q_per_kv
-    _check_slopes(slopes, heads, fused.device, what)
+    slopes_at = _check_slopes(slopes, heads, device, what)
     n = batch.n_seqs
     if batch.n_tokens != n or q_per_kv > Q8_MAX_HEADS or window < 0 or n_splits < 0:
         raise KernelError(f"{what} takes one token a sequence and at most {Q8_MAX_HEADS} query heads a K/V head")
-    cos, sin = rope if rope is not None else (None, None)
     L = lib()
-    if n_splits == 0:
-        pages = max_pages or batch.pages_stride
-        if window:
-            pages = min(pages, window // PAGE + 2)
-        with _on_device(fused):
-            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages)
-    parts, floats = _q8_parts(L, n, kv_heads, q_per_kv, head_dim, n_splits, fused.device)
-    out = torch.empty((n, heads * head_dim), dtype=fused.dtype, device=fused.device)
+    parts = parts_at = None
+    floats = 0
     with _on_device(fused):
-        _check(L.ptb_attention_decode_q8(_ptr(fused), _ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(out),
-                                         ctypes.byref(batch), _ptr(cos), _ptr(sin), pairs, 1 if interleaved else 0, _ptr(slopes),
-                                         heads, kv_heads, head_dim, ctypes.c_float(scale), int(window), 1 if write_cache else 0,
-                                         n_splits, _ptr(parts), ctypes.c_longlong(floats), _ptr(error_flag(fused.device)),
-                                         _stream(fused)), what)
+        if n_splits == 0:
+            pages = max_pages or batch.pages_stride
+            if window:
+                pages = min(pages, window // PAGE + 2)
+            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages, 1)
+        elif n_splits > 8:
+            n_splits = n_splits // 8 * 8
+        if n_splits > 8:
+            floats = L.ptb_attention_q8_floats(n, kv_heads, q_per_kv, head_dim, n_splits, 1)
+            parts = torch.empty(floats, dtype=torch.float32, device=fused.device)
+            parts_at = parts.data_ptr()
+        out = fused.new_empty((n, heads * head_dim))
+        _check(L.ptb_attention_decode_q8(fused.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(),
+                                         pool_pages, out.data_ptr(), ctypes.byref(batch), cos, sin, pairs, interleaved, slopes_at,
+                                         heads, kv_heads, head_dim, scale, window, write_cache, n_splits, parts_at, floats,
+                                         error_flag(fused.device).data_ptr(), _stream(fused)), what)
     return out
 
 
 def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
                  batch: StepBatchC, tile_seq: torch.Tensor, tile_q0: torch.Tensor, n_tiles: int, tile_tokens: int,
-                 slopes: Optional[torch.Tensor], kv_heads: int, scale: float, window: int = 0, n_pages: int = 0) -> torch.Tensor:
+                 slopes: Optional[torch.Tensor], kv_heads: int, scale: float, window: int = 0, n_pages: int = 0,
+                 n_splits: int = 0) -> torch.Tensor:
     """Causal attention of prompts and chunks over a cache in 8 bits that holds their keys and values already. ``q`` [tokens, heads,
     head_dim] bfloat16; tiles of ``tile_tokens`` consecutive new tokens as for the other prompt kernels. ``n_pages``: the pages that the
     step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of 64 or 128 take their
-    pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. Returns [tokens, heads * head_dim]."""
+    pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. ``n_splits``: as ``attention_decode_q8``
+    takes it, for the others. Returns [tokens, heads * head_dim]."""
     what = "attention_q8"
-    if not q.is_cuda or q.dtype != torch.bfloat16 or q.dim() != 3 or not q.is_contiguous() or q.shape[0] != batch.n_tokens:
+    if not (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 3 and q.is_contiguous() and q.shape[0] == batch.n_tokens):
         raise KernelError(f"{what} takes contiguous bfloat16 queries [tokens, heads, head_dim] of the step's tokens")
     n, heads, head_dim = q.shape
     if heads % kv_heads or window < 0:
         raise KernelError(f"{what}: {heads} heads on {kv_heads} K/V heads, window {window}")
-    _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, q.device, what)
-    _check_slopes(slopes, heads, q.device, what)
+    device = q.get_device()
+    pool_pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
+    slopes_at = _check_slopes(slopes, heads, device, what)
     for t in (tile_seq, tile_q0):
-        if t.dtype != torch.int32 or t.numel() < n_tiles or t.device != q.device or not t.is_contiguous():
+        if not (t.dtype is torch.int32 and t.numel() >= n_tiles and t.get_device() == device and t.is_contiguous()):
             raise KernelError(f"{what}: tile lists must be contiguous int32 tensors of {n_tiles} tiles on the queries' device")
     L = lib()
     if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and attention_tc_supports(head_dim) and not (slopes is not None and window):
         return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
                                       window, n_pages)
     rows = tile_tokens * (heads // kv_heads)
+    parts = parts_at = None
+    floats = 0
     with _on_device(q):
-        n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, min(batch.pages_stride, n_pages or batch.pages_stride))
-        parts, floats = _q8_parts(L, n_tiles, kv_heads, rows, head_dim, n_splits, q.device)
-        out = torch.empty((n, heads * head_dim), dtype=q.dtype, device=q.device)
-        _check(L.ptb_attention_q8(_ptr(q), _ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], _ptr(out),
-                                  ctypes.byref(batch), _ptr(tile_seq), _ptr(tile_q0), n_tiles, tile_tokens, _ptr(slopes), heads, kv_heads,
-                                  head_dim, ctypes.c_float(scale), int(window), n_splits, _ptr(parts), ctypes.c_longlong(floats),
-                                  _ptr(error_flag(q.device)), _stream(q)), what)
+        if n_splits == 0:
+            pages = batch.pages_stride if n_pages <= 0 else min(batch.pages_stride, n_pages)
+            n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, pages, 0)
+        elif n_splits > 8:
+            n_splits = n_splits // 8 * 8
+        if n_splits > 8:
+            floats = L.ptb_attention_q8_floats(n_tiles, kv_heads, rows, head_dim, n_splits, 0)
+            parts = torch.empty(floats, dtype=torch.float32, device=q.device)
+            parts_at = parts.data_ptr()
+        out = q.new_empty((n, heads * head_dim))
+        _check(L.ptb_attention_q8(q.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pool_pages,
+                                  out.data_ptr(), ctypes.byref(batch), tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, tile_tokens,
+                                  slopes_at, heads, kv_heads, head_dim, scale, window, n_splits, parts_at, floats,
+                                  error_flag(q.device).data_ptr(), _stream(q)), what)
     return out
 
 
@@ -1965,17 +1996,17 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
     # sizes in steps of an eighth: the prompt kernel keeps a tensor map for every size of pool
     step = max(1, 1 << max(0, n_pages.bit_length() - 3))
     room = (n_pages + step - 1) // step * step
-    tmp = torch.empty((2, room, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=device)
+    k, v = torch.empty((2, room, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=device).unbind(0)
     table = torch.empty((batch.n_seqs, batch.pages_stride), dtype=torch.int32, device=device)
     with _on_device(q):
-        _check(lib().ptb_unpack_q8(_ptr(k_pool), _ptr(k_exp), _ptr(v_pool), _ptr(v_exp), k_pool.shape[0], None, ctypes.byref(batch),
-                                   _ptr(table), n_pages, int(window), _ptr(tmp[0]), _ptr(tmp[1]), kv_heads, head_dim, head_dim,
-                                   _ptr(error_flag(device)), _stream(q)), "attention_q8 (pages)")
+        _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
+                                   ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
+                                   head_dim, error_flag(device).data_ptr(), _stream(q)), "attention_q8 (pages)")
         unpacked = StepBatchC.from_buffer_copy(batch)
         unpacked.pages = table.data_ptr()
         if slopes is not None:
-            return attention_tc(q, tmp[0], tmp[1], unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, slopes)
-        return attention_tc_extras(q, tmp[0], tmp[1], unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
+            return attention_tc(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, slopes)
+        return attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
 
 
 def copy_pages(pools, src, dst, out=None):
@@ -1983,28 +2014,33 @@ def copy_pages(pools, src, dst, out=None):
     or into the tensors ``out`` of the same types and page shapes (other storage, with pages of its own number). ``src`` and ``dst``:
     int32 NumPy arrays or sequences of page numbers; a source may be named often, a target once, and within one storage no page
     may be both. One launch for up to 960 pairs. Returns the tensors written to."""
-    into = list(pools) if out is None else list(out)
+    pools = list(pools)
+    into = pools if out is None else list(out)
     src, dst = np.ascontiguousarray(src, dtype=np.int32), np.ascontiguousarray(dst, dtype=np.int32)
     k = len(pools)
-    if k == 0 or k > 8 or len(into) != k or src.ndim != 1 or src.shape != dst.shape:
+    if not (0 < k <= 8 and len(into) == k and src.ndim == 1 and src.shape == dst.shape):
         raise KernelError("copy_pages takes one to eight tensors, as many targets and one target page for each source page")
-    args = []
+    t = pools[0]
+    device, n_src, n_dst = t.get_device(), t.shape[1], into[0].shape[1]
+    bases, page_bytes, entries = [], [], []
     for a, b in zip(pools, into):
-        if (a.dim() < 2 or not a.is_cuda or b.device != a.device or a.device != pools[0].device or a.dtype != b.dtype or a.shape[0] != b.shape[0]
-                or a.shape[2:] != b.shape[2:] or a.shape[1] != pools[0].shape[1] or b.shape[1] != into[0].shape[1]
-                or not a.is_contiguous() or not b.is_contiguous()):
+        shape = a.shape
+        if not (len(shape) >= 2 and a.get_device() == b.get_device() == device >= 0 and a.dtype is b.dtype and a.is_contiguous()
+                and b.is_contiguous() and shape[1] == n_src and (a is b or (b.shape[0] == shape[0] and b.shape[2:] == shape[2:]
+                                                                            and b.shape[1] == n_dst))):
             raise KernelError("copy_pages takes contiguous tensors [entries, pages, ...] on one CUDA device, all with the same number of "
                               "pages, and targets that differ in that number only")
-        page = a.element_size() * math.prod(a.shape[2:])
-        args.append((a.data_ptr(), b.data_ptr(), a.shape[1] * page, b.shape[1] * page, page, a.shape[0]))
-    ranges = [(p, p + n * e, q, q + m * e) for p, q, n, m, _, e in args]
-    if out is not None and any(lo < hi2 and lo2 < hi for lo, hi, _, _ in ranges for _, _, lo2, hi2 in ranges if lo < hi and lo2 < hi2):
+        bases.append((a.data_ptr(), b.data_ptr()))
+        page_bytes.append(a.element_size() * math.prod(shape[2:]))
+        entries.append(shape[0])
+    from_at, to_at = zip(*bases)
+    from_step, to_step = [n_src * p for p in page_bytes], [n_dst * p for p in page_bytes]
+    if out is not None and any(p < q + m * e and q < p + n * f for p, n, f in zip(from_at, from_step, entries)
+                               for q, m, e in zip(to_at, to_step, entries) if n * f and m * e):
         raise KernelError("copy_pages: the targets lie in the sources' memory")
-    col = list(zip(*args))
     pointers, numbers = ctypes.c_void_p * k, ctypes.c_longlong * k
-    t = pools[0]
     with _on_device(t):
-        _check(lib().ptb_copy_pages(pointers(*col[0]), pointers(*col[1]), numbers(*col[2]), numbers(*col[3]), numbers(*col[4]),
-                                    (ctypes.c_int * k)(*col[5]), k, ctypes.c_void_p(src.ctypes.data), ctypes.c_void_p(dst.ctypes.data),
-                                    ctypes.c_longlong(src.size), t.shape[1], into[0].shape[1], _stream(t)), "copy_pages")
+        _check(lib().ptb_copy_pages(pointers(*from_at), pointers(*to_at), numbers(*from_step), numbers(*to_step), numbers(*page_bytes),
+                                    (ctypes.c_int * k)(*entries), k, src.ctypes.data, dst.ctypes.data, src.size, n_src, n_dst,
+                                    _stream(t)), "copy_pages")
     return into
