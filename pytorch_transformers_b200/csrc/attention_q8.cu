@@ -15,8 +15,8 @@
 //
 // Pages land whole, keys and values, in rings that the tensor memory accelerator fills (2 requests a page: with boxes of 16 or
 // 32 rows, asked for by the warp that reads them or by one warp for all, the requests alone took 175 of 200 us where memory allows
-// 150). The warps of a ring take a share of a page's keys each, for one part of the rows or another; whoever is the last to have
-// read a page asks for the next one into its place. So no warp waits for another, but through a ring of pages, before the end. Which key and which entry an index of the
+// 150). The warps of a ring take a share of a page's keys each, for one part of the rows or another; they take turns to ask for the next page
+// into the place of one that all have read. So no warp waits for another, but through a ring of pages, before the end. Which key and which entry an index of the
 // matrix instruction stands for is free as long as both operands agree: a thread's share of a key's row is 16 codes in a row (a
 // 16-byte load gives four k-steps of fragments), and its share of a value's row likewise (columns of the output are
 // named accordingly, pairs of keys are put together with byte permutes). Nothing is transposed. The accelerator's swizzle and
@@ -200,8 +200,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   constexpr int TILE = Shape::TILE, KS = DP / 16, ST = TILE / 16;      // steps of 16 entries, of 16 keys
   constexpr bool Q_REGS = NH * DP <= 128;      // else the queries' fragments come from shared memory, tile by tile
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t bars[WARPS][MAX_STAGES];      // ring, stage: the page has landed
-  __shared__ int readers[WARPS][MAX_STAGES];                      // warps that have read it
+  __shared__ __align__(8) uint64_t bars[WARPS][2][MAX_STAGES];      // ring, stage: the page has landed; its warps have read it
   __shared__ __align__(16) unsigned char new_rows[2][DP];      // FUSED: the new token's codes, the page's exponents and whether one rose
   __shared__ int new_exp[2], new_rose[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nthreads = blockDim.x;
@@ -218,15 +217,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   int* row_exp = reinterpret_cast<int*>(smem + q_s + rows_pad * DP * 2);
   float* merged_ml = reinterpret_cast<float*>(row_exp + rows_pad);                  // [row][2]
   const int D = p.dim, qpk = p.heads / p.kv_heads;
-  const uint32_t bar0 = smem_u32(&bars[ring_no < WARPS ? ring_no : 0][0]);
+  const uint32_t bar0 = smem_u32(&bars[ring_no < WARPS ? ring_no : 0][0][0]);      // 8 * MAX_STAGES on: read
   const bool leads = !idle && warp == ring_no * p.row_groups * p.page_parts;      // its first lane asks for the first pages
-  if (leads && lane == 0) {
-    for (int st = 0; st < p.stages; ++st) {
-      mbar_init(bar0 + 8 * st, 1);
-      readers[ring_no][st] = 0;
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-  }
   pdl_entry();
 
   // this block's rows: row r of the block is head (row0 + r) % qpk of the group and token (row0 + r) / qpk of the tile
@@ -250,10 +242,10 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   const int split = blockIdx.z;
   // pages of this block (whole ones: the page that a step appends to has one reader), and of them this warp's tiles
   const int pg0 = low / PTB_PAGE, n_pages = last_pos / PTB_PAGE + 1 - pg0;
-  auto share = [&](int i) {
+  auto up_to = [&](int i) {
     return n_pages < (1 << 21) ? i * n_pages / p.n_splits : int((long long)i * n_pages / p.n_splits);      // n_splits <= 512
   };
-  const int pg_begin = pg0 + (p.n_splits == 1 ? 0 : share(split)), pg_end = pg0 + (p.n_splits == 1 ? n_pages : share(split + 1));
+  const int pg_begin = pg0 + (p.n_splits == 1 ? 0 : up_to(split)), pg_end = pg0 + (p.n_splits == 1 ? n_pages : up_to(split + 1));
   const bool appends = FUSED && p.write_cache && pg_end == pg0 + n_pages && pg_begin < pg_end;
   const int fused_width = p.kv_heads * (qpk + 2) * D;
 
@@ -277,11 +269,6 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   };
   int page_now, exps_now, page_next = 0, exps_next = 0;
   look_up(0, page_now, exps_now);
-  int page_ahead = page_now;      // of the stretch that pages are asked for from
-  auto page_of = [&](int i) {      // by every lane, for i one after another
-    if ((i & 31) == 0 && i > 0) page_ahead = page_next;
-    return __shfl_sync(0xffffffffu, page_ahead, i & 31);
-  };
   auto ask = [&](int page, int st) {      // by one thread
     const uint32_t bar = bar0 + 8 * st, to = smem_u32(smem) + ring + st * Shape::STAGE_BYTES;
     const int y = (page * p.kv_heads + g) * PTB_PAGE;
@@ -293,11 +280,21 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   };
   auto ask_first = [&]() {
     for (int st = 0; st < p.stages && st < n_mine; ++st) {
-      const int page = page_of(st);
+      const int page = __shfl_sync(0xffffffffu, page_now, st);
       if (lane == 0) ask(page, st);
     }
   };
-  if (leads) ask_first();      // on their way while the queries are made
+  if (leads) {      // on their way while the queries are made
+    if (lane == 0) {
+      for (int st = 0; st < p.stages; ++st) {
+        mbar_init(bar0 + 8 * st, 1);
+        mbar_init(bar0 + 8 * (MAX_STAGES + st), sharers);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncwarp();
+    ask_first();
+  }
   if (appends) {
     const int page = pages[pg_end - 1];
     const __nv_bfloat16* frow = p.rows + size_t(start) * fused_width + size_t(g) * (qpk + 2) * D;
@@ -426,18 +423,28 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     v_at[u] = ring + PTB_PAGE * DP + (DP == 64 ? place<DP>(kappa<DP>(2 * t4 + u), g4 >> 1) + (g4 & 1) * 8 : place<DP>(kappa<DP>(2 * t4 + u), g4));
   constexpr int EIGHT = 8 * (DP == 64 ? 64 : 128);      // bytes from a row to that of eight keys on
   const int part_keys = PTB_PAGE / p.page_parts;
-  int st = 0;
+  int st = 0, reads_turn = 0;
 
   int i = 0;
   for (; i < n_mine && alive; ++i) {
-    const int i_ahead = i + p.stages;
-    const int page_ahead_now = i_ahead < n_mine ? page_of(i_ahead) : 0;
-    if ((i & 31) == 0 && i > 0) exps_now = exps_next;
+    if ((i & 31) == 0 && i > 0) {
+      page_now = page_next;
+      exps_now = exps_next;
+    }
     if ((i & 31) == 8 && (i & ~31) + 32 < n_mine) look_up((i >> 5) + 1, page_next, exps_next);
     const int both = __shfl_sync(0xffffffffu, exps_now, i & 31);
     const int page_key0 = (pg_begin + ring_no + i * p.rings) * PTB_PAGE;
     landed(i, st, turn & 1);
     if (!alive) break;
+    // page `stages` on from the one before, into its place: its warps take turns to ask, a page late, when all have read it
+    if (i > 0 && i - 1 + p.stages < n_mine && rg == 0 && (i - 1) % p.page_parts == part) {
+      const int j = i - 1 + p.stages, before = st == 0 ? p.stages - 1 : st - 1;
+      const int page = __shfl_sync(0xffffffffu, (j ^ i) < 32 ? page_now : page_next, j & 31);
+      const uint32_t bar = bar0 + 8 * (MAX_STAGES + before), parity = (st == 0 ? reads_turn - 1 : reads_turn) & 1;
+      if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 23));
+      if (!alive) break;
+      if (lane == 0) ask(page, before);
+    }
     const int first_key = page_key0 + part * part_keys;
     if (FUSED && appends && past - first_key >= 0 && past - first_key < part_keys) {
       // the new token's codes from this block rather than from the page, where they may have come after the copy; all who read them
@@ -629,17 +636,9 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
         }
       }
     }
-    // the last warp to have read the page asks for the next one in its place
     __syncwarp();
-    if (i_ahead < n_mine && lane == 0) {
-      __threadfence_block();
-      if (atomicAdd(&readers[ring_no][st], 1) == sharers - 1) {
-        readers[ring_no][st] = 0;
-        __threadfence_block();
-        ask(page_ahead_now, st);
-      }
-    }
-    if (++st == p.stages) st = 0, ++turn;
+    if (lane == 0) mbar_arrive(bar0 + 8 * (MAX_STAGES + st));
+    if (++st == p.stages) st = 0, ++turn, ++reads_turn;
   }
   if (!alive)      // a wait ran out: what is in flight lands before the block ends (bounded waits again)
     for (int k = 0; k < p.stages && i + k < n_mine; ++k) {
@@ -664,21 +663,25 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
       if (g4 == 0 && !idle) *reinterpret_cast<float2*>(join_ml + 2 * r) = make_float2(m_run[n][h], l);
     }
   __syncthreads();      // and the rings are done with
+  for (int r = tid; r < n_rows; r += WARPS * 32) {
+    float m = -INFINITY, l = 0.f;
+    for (int k = 0; k < key_groups; ++k) m = fmaxf(m, join_ml[2 * (k * rows_pad + r)]);
+    for (int k = 0; k < key_groups; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(join_ml + 2 * (k * rows_pad + r));
+      l += ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.y * exp2f(ml.x - m);
+    }
+    *reinterpret_cast<float2*>(merged_ml + 2 * r) = make_float2(m, l);
+  }
+  __syncthreads();
 #pragma unroll
   for (int n = 0; n < NH; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int r = (rg * NH + n) * 8 + 2 * t4 + h;
       if (r >= n_rows || idle) continue;
-      float m = -INFINITY, l = 0.f;
-      for (int k = 0; k < key_groups; ++k) m = fmaxf(m, join_ml[2 * (k * rows_pad + r)]);
-      for (int k = 0; k < key_groups; ++k) {
-        const float2 ml = *reinterpret_cast<const float2*>(join_ml + 2 * (k * rows_pad + r));
-        l += ml.x == -INFINITY && ml.y == 0.f ? 0.f : ml.y * exp2f(ml.x - m);
-      }
-      if (kg == 0 && g4 == 0) *reinterpret_cast<float2*>(merged_ml + 2 * r) = make_float2(m, l);
+      const float2 ml = *reinterpret_cast<const float2*>(merged_ml + 2 * r);
       const bool none = m_run[n][h] == -INFINITY && l_run[n][h] == 0.f;
-      const float part = none ? 0.f : exp2f(m_run[n][h] - m) / l * power_of_two(unit);
+      const float share = none ? 0.f : exp2f(m_run[n][h] - ml.x) / ml.y * power_of_two(unit);
       constexpr int COLS = DP == 64 ? 8 : 16;      // entries of a row of the output that a thread holds: [g4][COLS]
       float* to = join + size_t(kg * rows_pad + r) * Shape::PITCH + g4 * COLS;
 #pragma unroll
@@ -687,7 +690,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
         for (int c = 0; c < COLS / 2; c += 2) {
           const float(&x)[4] = o[n][rr * 8 + c], (&y)[4] = o[n][rr * 8 + c + 1];
           *reinterpret_cast<float4*>(to + rr * 128 + 2 * c) =
-              none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[h] * part, x[2 + h] * part, y[h] * part, y[2 + h] * part);
+              none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[h] * share, x[2 + h] * share, y[h] * share, y[2 + h] * share);
         }
     }
   __syncthreads();
@@ -887,15 +890,16 @@ bool known(int heads, int kv_heads, int dim, int pool_pages) {
   return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && kv_heads <= 65535 && dim >= 16 && dim <= 256 && dim % 16 == 0 && pool_pages > 0 &&
          (long long)pool_pages * kv_heads * PTB_PAGE < (1ll << 31);      // rows of codes, as the copies count them
 }
-// Blocks that share a row's pages: about two waves of them on the SMs in all, each with four pages at least. Up to eight form a cluster
-// and join through its shared memory; more are a multiple of eight, whose clusters join through a workspace.
+// Blocks that share a row's pages: as many as the SMs take at a time, two pages each at least. Up to eight form a cluster and join
+// through its shared memory; more are a multiple of eight, of eight pages each at least, whose clusters join through a workspace.
 int splits_of(long long blocks, int pages, int dp, int nh) {
   const long long slots = (nh == 4 || dp == 256 ? 1ll : 2ll) * sm_count();
-  long long want = (2 * slots + blocks - 1) / (blocks > 0 ? blocks : 1);
-  if (blocks >= 8 * slots) want = 1;
-  const long long most = pages / 4;
-  if (want > most) want = most;
-  if (want > MAX_CLUSTER) want = want / MAX_CLUSTER * MAX_CLUSTER;
+  long long want = blocks > 0 ? slots / blocks : 1;
+  if (want > pages / 2) want = pages / 2;
+  if (want > MAX_CLUSTER) {
+    const long long wide = (want < pages / 8 ? want : pages / 8) / MAX_CLUSTER * MAX_CLUSTER;
+    want = wide > MAX_CLUSTER ? wide : MAX_CLUSTER;
+  }
   return int(want < 1 ? 1 : want > 512 ? 512 : want);
 }
 int teams_of(int n_splits) { return n_splits <= MAX_CLUSTER ? 1 : n_splits / MAX_CLUSTER; }
