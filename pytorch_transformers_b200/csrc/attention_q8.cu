@@ -437,7 +437,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     landed(i, st, turn & 1);
     if (!alive) break;
     // page `stages` on from the one before, into its place: its warps take turns to ask, a page late, when all have read it
-    if (i > 0 && i - 1 + p.stages < n_mine && rg == 0 && (i - 1) % p.page_parts == part) {
+    if (i > 0 && i - 1 + p.stages < n_mine && rg == 0 && ((i - 1) & (p.page_parts - 1)) == part) {      // page_parts is a power of two
       const int j = i - 1 + p.stages, before = st == 0 ? p.stages - 1 : st - 1;
       const int page = __shfl_sync(0xffffffffu, (j ^ i) < 32 ? page_now : page_next, j & 31);
       const uint32_t bar = bar0 + 8 * (MAX_STAGES + before), parity = (st == 0 ? reads_turn - 1 : reads_turn) & 1;
@@ -791,11 +791,11 @@ struct Plan {
   int dp, nh, row_groups, page_parts, rings, stages, rows_pad;
 };
 // rows: of a block's tile at most (more are divided among blocks)
-Plan plan_of(int dim, int rows, bool fused) {
+Plan plan_of(int dim, int rows) {
   Plan q;
   q.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
   q.nh = rows <= 8 ? 1 : rows <= 16 || q.dp == 256 ? 2 : 4;
-  const int groups = (rows + 8 * q.nh - 1) / (8 * q.nh), most = q.dp == 256 ? 8 : q.dp == 128 && !fused ? 2 : 4;
+  const int groups = (rows + 8 * q.nh - 1) / (8 * q.nh), most = q.dp == 256 ? 8 : 4;
   q.row_groups = groups < most ? groups : most;
   q.rows_pad = q.row_groups * 8 * q.nh;
   const int keys = WARPS / q.row_groups, parts = q.dp == 64 ? 2 : 4;      // a part is a tile at least
@@ -908,13 +908,13 @@ bool splits_known(int n_splits) { return n_splits >= 1 && n_splits <= 512 && (n_
 
 // How many blocks share a row's pages (n_splits below: 1 to 8, or a multiple of 8) and the floats of workspace that they need: rows = query heads of a K/V head times
 // tokens of a tile; tiles = sequences of a step of single tokens, or tiles of a prompt; pages: that a row may see, at most.
-PTB_API int ptb_attention_q8_splits(int tiles, int kv_heads, int rows, int dim, int pages, int fused) {
-  const Plan q = plan_of(dim, rows, fused != 0);
+PTB_API int ptb_attention_q8_splits(int tiles, int kv_heads, int rows, int dim, int pages) {
+  const Plan q = plan_of(dim, rows);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
   return splits_of((long long)tiles * kv_heads * chunks, pages, q.dp, q.nh);
 }
-PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int dim, int n_splits, int fused) {
-  const Plan q = plan_of(dim, rows, fused != 0);
+PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int dim, int n_splits) {
+  const Plan q = plan_of(dim, rows);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
   const int teams = teams_of(n_splits);
   return teams > 1 ? (long long)tiles * kv_heads * chunks * teams * q.rows_pad * (dim + 2) : 0;
@@ -931,13 +931,13 @@ PTB_API int ptb_attention_decode_q8(const void* fused, void* k_pool, void* k_exp
       window < 0 || !splits_known(n_splits) || error_flag == nullptr || (rot_pairs > 0 && (rope_cos == nullptr || rope_sin == nullptr)))
     return PTB_ERR_SIZE;
   if (!aligned16(fused) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
-  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, heads / kv_heads, dim, n_splits, 1) > part_floats) return PTB_ERR_SIZE;
+  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, heads / kv_heads, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
   AttnQ8 p = {};
   p.rows = (const __nv_bfloat16*)fused; p.k_pool = (uint8_t*)k_pool; p.v_pool = (uint8_t*)v_pool; p.k_exp = (int8_t*)k_exp;
   p.v_exp = (int8_t*)v_exp; p.out = (__nv_bfloat16*)out; p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.slopes = slopes;
   p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pool_pages = pool_pages; p.rot_pairs = rot_pairs; p.interleaved = interleaved;
   p.write_cache = write_cache; p.window = window; p.n_splits = n_splits; p.scale = scale; p.parts = parts; p.error_flag = error_flag;
-  const Plan q = plan_of(dim, heads / kv_heads, true);
+  const Plan q = plan_of(dim, heads / kv_heads);
   p.row_groups = q.row_groups; p.page_parts = q.page_parts; p.rings = q.rings; p.stages = q.stages;
   p.teams = teams_of(n_splits); p.cluster = n_splits / p.teams;
   return launch_any<true>(*sb, p, q, dim3(sb->n_seqs, kv_heads, n_splits), stream);
@@ -955,8 +955,8 @@ PTB_API int ptb_attention_q8(const void* q_rows, const void* k_pool, const void*
     return PTB_ERR_SIZE;
   if (!aligned16(q_rows) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
   const int rows = tile_tokens * (heads / kv_heads);
-  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, dim, n_splits, 0) > part_floats) return PTB_ERR_SIZE;
-  const Plan q = plan_of(dim, rows, false);
+  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
+  const Plan q = plan_of(dim, rows);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
   if (chunks * kv_heads > 65535) return PTB_ERR_SIZE;
   AttnQ8 p = {};

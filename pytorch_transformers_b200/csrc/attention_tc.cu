@@ -1091,3 +1091,21 @@ PTB_API int ptb_attention_tc_extras(const void* q, const void* k_pool, const voi
   return wide_weights ? PTB_TCX(192, 128, true) : PTB_TCX(192, 128, false);
 #undef PTB_TCX
 }
+
+// A window beside per-head score slopes, weights of two terms, heads of 64 or 128 alike (prompts over a cache in 8 bits).
+PTB_API int ptb_attention_tc_extras_biased(const void* q, const void* k_pool, const void* v_pool, int pool_pages, void* out,
+                                           const StepBatch* sb, const int* tile_seq, const int* tile_q0, int n_tiles, const float* slopes,
+                                           int heads, int kv_heads, int head_dim, float scale, int window, int* error_flag,
+                                           cudaStream_t stream) {
+  if (n_tiles <= 0) return PTB_OK;
+  if (pool_pages <= 0 || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(q) || !aligned16(out)) return PTB_ERR_ALIGN;
+  if (!ptb_attention_tc_supports(head_dim) || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || n_tiles > 65535 ||
+      error_flag == nullptr || window < 0 || slopes == nullptr)
+    return PTB_ERR_SIZE;
+  TcParams p = {};
+  p.heads = heads; p.kv_heads = kv_heads; p.scale = scale; p.slopes = slopes; p.window = window; p.out_scale = 1.f;
+  p.out_stride = heads * head_dim;
+  return head_dim == 64
+             ? launch_tc<64, 64, true, true, true>(q, k_pool, v_pool, pool_pages, out, *sb, tile_seq, tile_q0, n_tiles, p, error_flag, stream)
+             : launch_tc<128, 128, true, true, true>(q, k_pool, v_pool, pool_pages, out, *sb, tile_seq, tile_q0, n_tiles, p, error_flag, stream);
+}

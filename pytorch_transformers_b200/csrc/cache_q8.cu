@@ -25,7 +25,8 @@ struct StoreParams {
   int* error_flag;
 };
 
-__global__ void __launch_bounds__(STORE_THREADS) store_q8_kernel(StepBatch sb, StoreParams p) {
+// MOST: eighths of a page's rows that a thread holds (4 for heads up to 128, 8 up to 256)
+template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_kernel(StepBatch sb, StoreParams p) {
   pdl_entry();
   __shared__ float scratch[32];
   const int tid = threadIdx.x, eighths = p.dim / 8, rows = p.q_per_kv + 2;
@@ -68,7 +69,6 @@ __global__ void __launch_bounds__(STORE_THREADS) store_q8_kernel(StepBatch sb, S
   int8_t* exps = (keys ? p.k_exp : p.v_exp) + block;
   const int old = *exps;
   const __nv_bfloat16* src = p.fused + size_t(g * rows + p.q_per_kv + (keys ? 0 : 1)) * p.dim;
-  constexpr int MOST = PTB_PAGE * 256 / 8 / STORE_THREADS;      // eighths of rows a thread holds
   const int total = (last - first) * eighths;
   float x[MOST][8];
   float most = 0.f;
@@ -175,6 +175,17 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
   }
 }
 
+// ------------------------------------------------------------------------------------------------ heads of other sizes
+// Rows of `from` entries as rows of `to` entries, zero past `from`, or cut to `to`: heads that the tcgen05 prompt kernel does not take go through it as
+// heads of 64 or 128. A thread moves 16 bytes.
+__global__ void __launch_bounds__(256) pitch_rows_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst, long long rows, int from, int to) {
+  pdl_entry();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long r = i / to;
+  const int c = int(i - r * to);
+  if (r < rows) dst[i] = c < from ? src[r * from + c] : make_uint4(0, 0, 0, 0);
+}
+
 // ------------------------------------------------------------------------------------------------ copies
 // Pages of several tensors [entries][pages][page bytes] in one launch. The pairs travel as the kernel's parameters: no copy of
 // them to the device, none of their memory to keep until the kernel has run.
@@ -259,7 +270,9 @@ PTB_API int ptb_store_q8(const void* fused, void* q_out, void* k_pool, void* k_e
   p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.rot_pairs = rot_pairs; p.interleaved = interleaved;
   p.kv_heads = kv_heads; p.q_per_kv = q_per_kv; p.dim = dim; p.pool_pages = pool_pages; p.page_blocks = int(page_blocks);
   p.error_flag = error_flag;
-  launch_pdl(store_q8_kernel, dim3(unsigned(page_blocks + q_blocks)), dim3(STORE_THREADS), 0, stream, *sb, p);
+  const dim3 grid(unsigned(page_blocks + q_blocks)), block(STORE_THREADS);
+  if (dim <= 128) launch_pdl(store_q8_kernel<4>, grid, block, 0, stream, *sb, p);
+  else launch_pdl(store_q8_kernel<8>, grid, block, 0, stream, *sb, p);
   return launch_status();
 }
 
@@ -279,6 +292,16 @@ PTB_API int ptb_unpack_q8(const void* k_pool, const void* k_exp, const void* v_p
   p.kv_heads = kv_heads; p.dim = dim; p.out_dim = out_dim; p.pool_pages = pool_pages; p.window = window; p.error_flag = error_flag;
   StepBatch none = {};
   launch_pdl(unpack_q8_kernel, dim3(n_pages, kv_heads), dim3(256), 0, stream, sb ? *sb : none, p);
+  return launch_status();
+}
+
+// `rows` rows of from_dim bfloat16 entries into rows of to_dim (multiples of 8), padded with zeros or cut.
+PTB_API int ptb_pitch_rows(const void* src, void* dst, long long rows, int from_dim, int to_dim, cudaStream_t stream) {
+  if (rows <= 0) return PTB_OK;
+  if (from_dim <= 0 || to_dim <= 0 || from_dim % 8 != 0 || to_dim % 8 != 0 || rows * (to_dim / 8) > (1ll << 38)) return PTB_ERR_SIZE;
+  if (!aligned16(src) || !aligned16(dst)) return PTB_ERR_ALIGN;
+  launch_pdl(pitch_rows_kernel, dim3(unsigned((rows * (to_dim / 8) + 255) / 256)), dim3(256), 0, stream, (const uint4*)src, (uint4*)dst, rows,
+             from_dim / 8, to_dim / 8);
   return launch_status();
 }
 

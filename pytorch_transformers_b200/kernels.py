@@ -120,7 +120,8 @@ def lib():
                      "ptb_head_norm_gate_act", "ptb_gla_decay", "ptb_gla_walk", "ptb_gla_chunks", "ptb_gla_max_dim",
                      "ptb_gla_chunk_tokens", "ptb_delta_prepare", "ptb_delta_walk", "ptb_delta_chunks",
                      "ptb_delta_chunks_supports", "ptb_post_norm", "ptb_token_gate", "ptb_round_rows", "ptb_route_biased", "ptb_attention_tc_sizes", "ptb_attention_tc_supports_sizes", "ptb_attention_tc_extras",
-                     "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_q8_splits", "ptb_attention_decode_q8", "ptb_attention_q8"):
+                     "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_q8_splits", "ptb_attention_decode_q8", "ptb_attention_q8",
+                     "ptb_attention_tc_extras_biased", "ptb_pitch_rows"):
             getattr(L, name).restype = ctypes.c_int
         L.ptb_latent_part_floats.restype = ctypes.c_longlong
         L.ptb_rglru_chunks_work_floats.restype = ctypes.c_longlong
@@ -131,8 +132,10 @@ def lib():
         P, I, N, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
         L.ptb_store_q8.argtypes = [P] * 6 + [I, P, P, P] + [I] * 5 + [P, P]
         L.ptb_unpack_q8.argtypes = [P] * 4 + [I, P, P, P, I, I, P, P, I, I, I, P, P]
-        L.ptb_attention_q8_splits.argtypes = [I] * 6
-        L.ptb_attention_q8_floats.argtypes = [I] * 6
+        L.ptb_attention_q8_splits.argtypes = [I] * 5
+        L.ptb_attention_q8_floats.argtypes = [I] * 5
+        L.ptb_pitch_rows.argtypes = [P, P, N, I, I, P]
+        L.ptb_attention_tc_extras_biased.argtypes = [P] * 3 + [I, P, P, P, P, I, P, I, I, I, F, I, P, P]
         L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, P, N, P, P]
         L.ptb_attention_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, P, N, P, P]
         L.ptb_copy_pages.argtypes = [P] * 6 + [I, P, P, N, I, I, P]
@@ -1897,7 +1900,7 @@ def unpack_pages_q8(k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Ten
     _, kv_heads, _, head_dim = k_pool.shape
     pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, ids.get_device(), "unpack_pages_q8")
     n = ids.numel()
-    k, v = torch.empty((2, n, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device).unbind(0)
+    k, v = (torch.empty((n, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device) for _ in range(2))
     with _on_device(ids):
         _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pages, ids.data_ptr(), None,
                                    None, n, 0, k.data_ptr(), v.data_ptr(), kv_heads, head_dim, head_dim,
@@ -1930,11 +1933,11 @@ def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.
             pages = max_pages or batch.pages_stride
             if window:
                 pages = min(pages, window // PAGE + 2)
-            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages, 1)
+            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages)
         elif n_splits > 8:
             n_splits = n_splits // 8 * 8
         if n_splits > 8:
-            floats = L.ptb_attention_q8_floats(n, kv_heads, q_per_kv, head_dim, n_splits, 1)
+            floats = L.ptb_attention_q8_floats(n, kv_heads, q_per_kv, head_dim, n_splits)
             parts = torch.empty(floats, dtype=torch.float32, device=fused.device)
             parts_at = parts.data_ptr()
         out = fused.new_empty((n, heads * head_dim))
@@ -1951,7 +1954,7 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
                  n_splits: int = 0) -> torch.Tensor:
     """Causal attention of prompts and chunks over a cache in 8 bits that holds their keys and values already. ``q`` [tokens, heads,
     head_dim] bfloat16; tiles of ``tile_tokens`` consecutive new tokens as for the other prompt kernels. ``n_pages``: the pages that the
-    step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of 64 or 128 take their
+    step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of up to 128 take their
     pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. ``n_splits``: as ``attention_decode_q8``
     takes it, for the others. Returns [tokens, heads * head_dim]."""
     what = "attention_q8"
@@ -1967,7 +1970,7 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
         if not (t.dtype is torch.int32 and t.numel() >= n_tiles and t.get_device() == device and t.is_contiguous()):
             raise KernelError(f"{what}: tile lists must be contiguous int32 tensors of {n_tiles} tiles on the queries' device")
     L = lib()
-    if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and attention_tc_supports(head_dim) and not (slopes is not None and window):
+    if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and head_dim <= 128:
         return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
                                       window, n_pages)
     rows = tile_tokens * (heads // kv_heads)
@@ -1976,11 +1979,11 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     with _on_device(q):
         if n_splits == 0:
             pages = batch.pages_stride if n_pages <= 0 else min(batch.pages_stride, n_pages)
-            n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, pages, 0)
+            n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, pages)
         elif n_splits > 8:
             n_splits = n_splits // 8 * 8
         if n_splits > 8:
-            floats = L.ptb_attention_q8_floats(n_tiles, kv_heads, rows, head_dim, n_splits, 0)
+            floats = L.ptb_attention_q8_floats(n_tiles, kv_heads, rows, head_dim, n_splits)
             parts = torch.empty(floats, dtype=torch.float32, device=q.device)
             parts_at = parts.data_ptr()
         out = q.new_empty((n, heads * head_dim))
@@ -1992,21 +1995,35 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
 
 
 def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale, window, n_pages):
-    head_dim, device = q.shape[2], q.device
+    n, heads, head_dim = q.shape
+    device, wide = q.device, 64 if head_dim <= 64 else 128      # heads of other sizes as heads of these, with zeros
     # sizes in steps of an eighth: the prompt kernel keeps a tensor map for every size of pool
     step = max(1, 1 << max(0, n_pages.bit_length() - 3))
     room = (n_pages + step - 1) // step * step
-    k, v = torch.empty((2, room, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=device).unbind(0)
+    k, v = (torch.empty((room, kv_heads, PAGE, wide), dtype=torch.bfloat16, device=device) for _ in range(2))
     table = torch.empty((batch.n_seqs, batch.pages_stride), dtype=torch.int32, device=device)
+    L, flag = lib(), error_flag(device).data_ptr()
     with _on_device(q):
-        _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
-                                   ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
-                                   head_dim, error_flag(device).data_ptr(), _stream(q)), "attention_q8 (pages)")
+        stream = _stream(q)
+        _check(L.ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
+                               ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
+                               wide, flag, stream), "attention_q8 (pages)")
         unpacked = StepBatchC.from_buffer_copy(batch)
         unpacked.pages = table.data_ptr()
-        if slopes is not None:
-            return attention_tc(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, slopes)
-        return attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
+        if wide != head_dim:
+            own, q = q, q.new_empty((n, heads, wide))
+            _check(L.ptb_pitch_rows(own.data_ptr(), q.data_ptr(), n * heads, head_dim, wide, stream), "attention_q8 (queries)")
+        if slopes is None:
+            out = attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
+        else:
+            out = q.new_empty((n, heads * wide))
+            _check(L.ptb_attention_tc_extras_biased(q.data_ptr(), k.data_ptr(), v.data_ptr(), room, out.data_ptr(), ctypes.byref(unpacked),
+                                                    tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, slopes.data_ptr(), heads, kv_heads,
+                                                    wide, scale, window, flag, stream), "attention_q8 (prompt)")
+        if wide != head_dim:
+            padded, out = out, q.new_empty((n, heads * head_dim))
+            _check(L.ptb_pitch_rows(padded.data_ptr(), out.data_ptr(), n * heads, wide, head_dim, stream), "attention_q8 (result)")
+    return out
 
 
 def copy_pages(pools, src, dst, out=None):

@@ -388,6 +388,18 @@ def test_prompts_unpacked(K, kv, qpk, dim, slopes, pasts, news):
     c.check(out, q, weight_bits=7 if slopes else 11)
 
 
+@pytest.mark.parametrize("kv,qpk,dim", [(1, 5, 16), (2, 3, 48), (3, 2, 96), (1, 7, 112), (2, 2, 64), (1, 4, 128)])
+@pytest.mark.parametrize("slopes,window", [(False, 0), (True, 0), (False, 130), (True, 130)])
+def test_prompts_unpacked_of_other_heads(K, kv, qpk, dim, slopes, window):
+    # heads that the prompt kernel takes as 64 or 128 entries, and slopes beside a window; weights of two terms throughout
+    pasts, news = [0, 300, 64], [131, 200, 3]
+    c = Case(kv, qpk, dim, pasts, news, slopes=slopes, window=window, seed=dim + qpk, spread=2.0)
+    if window:
+        c.give_back_left_of_windows()
+    out, q = run_prompt(K, c, sum((p + n + PAGE - 1) // PAGE for p, n in zip(pasts, news)))
+    c.check(out, q)
+
+
 # ------------------------------------------------------------------------------------------------ graphs and streams
 def test_captured_and_replayed_on_another_stream(K):
     c = Case(2, 4, 64, [100, 2000], [1, 1], rot=64, seed=9)
