@@ -279,17 +279,12 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     for (int x = 0; x < DP; x += 128) tma_load_2d(to + PTB_PAGE * DP + x * PTB_PAGE, &v_map, x, y, bar);
   };
   auto ask_first = [&]() {
-    for (int st = 0; st < p.stages && st < n_mine; ++st) {
-      const int page = __shfl_sync(0xffffffffu, page_now, st);
-      if (lane == 0) ask(page, st);
-    }
+    if (lane < p.stages && lane < n_mine) ask(page_now, lane);      // a lane a stage
   };
   if (leads) {      // on their way while the queries are made
-    if (lane == 0) {
-      for (int st = 0; st < p.stages; ++st) {
-        mbar_init(bar0 + 8 * st, 1);
-        mbar_init(bar0 + 8 * (MAX_STAGES + st), sharers);
-      }
+    if (lane < p.stages) {
+      mbar_init(bar0 + 8 * lane, 1);
+      mbar_init(bar0 + 8 * (MAX_STAGES + lane), sharers);
       asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncwarp();
@@ -298,8 +293,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   if (appends) {
     const int page = pages[pg_end - 1];
     const __nv_bfloat16* frow = p.rows + size_t(start) * fused_width + size_t(g) * (qpk + 2) * D;
-    if (warp < 2) {
-      const int which = warp;
+    if (warp == 5 || warp == 7) {      // never the ones that ask for the first pages
+      const int which = warp == 7;
       bool rose = false;
       int e = 0;
       if (page >= 0 && page < p.pool_pages) {
@@ -902,42 +897,49 @@ int splits_of(long long blocks, int pages, int dp, int nh) {
   }
   return int(want < 1 ? 1 : want > 512 ? 512 : want);
 }
+enum { PTB_NEEDS_WORKSPACE = -1 };
 int teams_of(int n_splits) { return n_splits <= MAX_CLUSTER ? 1 : n_splits / MAX_CLUSTER; }
 bool splits_known(int n_splits) { return n_splits >= 1 && n_splits <= 512 && (n_splits <= MAX_CLUSTER || n_splits % MAX_CLUSTER == 0); }
 }  // namespace
 
-// How many blocks share a row's pages (n_splits below: 1 to 8, or a multiple of 8) and the floats of workspace that they need: rows = query heads of a K/V head times
-// tokens of a tile; tiles = sequences of a step of single tokens, or tiles of a prompt; pages: that a row may see, at most.
-PTB_API int ptb_attention_q8_splits(int tiles, int kv_heads, int rows, int dim, int pages) {
-  const Plan q = plan_of(dim, rows);
-  const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
-  return splits_of((long long)tiles * kv_heads * chunks, pages, q.dp, q.nh);
+// Blocks that share a row's pages where the caller leaves it open (n_splits 0). rows: query heads of a K/V head times tokens of a tile, at most;
+// pages: that a row may see, at most. Prompts' last tiles are seldom full: as many chunks of rows are counted as the step's tokens fill.
+static int splits_or(int n_splits, int tiles, int kv_heads, int rows, int tile_tokens, int pages, int tokens, const Plan& q) {
+  if (n_splits > 0) return n_splits;
+  const long long chunks = ((long long)rows / tile_tokens * tokens + q.rows_pad - 1) / q.rows_pad;
+  return splits_of(kv_heads * (chunks > tiles ? chunks : tiles), pages, q.dp, q.nh);
 }
-PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int dim, int n_splits) {
+
+// Floats of workspace (`parts` below) of a call that answered PTB_NEEDS_WORKSPACE, for the same sizes; tokens: of the step.
+PTB_API long long ptb_attention_q8_floats(int tiles, int kv_heads, int rows, int tile_tokens, int dim, int n_splits, int pages, int tokens) {
   const Plan q = plan_of(dim, rows);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
-  const int teams = teams_of(n_splits);
+  const int teams = teams_of(splits_or(n_splits, tiles, kv_heads, rows, tile_tokens, pages, tokens, q));
   return teams > 1 ? (long long)tiles * kv_heads * chunks * teams * q.rows_pad * (dim + 2) : 0;
 }
 
 // A step of single tokens. fused [n_seqs, kv_heads * (heads / kv_heads + 2) * dim] bfloat16, out [n_seqs, heads * dim]; pools and exponents as
-// in cache_q8.cu. At most 128 query heads a K/V head.
+// in cache_q8.cu. At most 128 query heads a K/V head. n_splits: 1 to 8, a multiple of 8, or 0 for a choice by the sizes and
+// `pages`, the most that a sequence spans. PTB_NEEDS_WORKSPACE: nothing was launched, and `parts` has to have ptb_attention_q8_floats floats.
 PTB_API int ptb_attention_decode_q8(const void* fused, void* k_pool, void* k_exp, void* v_pool, void* v_exp, int pool_pages, void* out,
                                     const StepBatch* sb, const float* rope_cos, const float* rope_sin, int rot_pairs, int interleaved,
                                     const float* slopes, int heads, int kv_heads, int dim, float scale, int window, int write_cache,
-                                    int n_splits, float* parts, long long part_floats, int* error_flag, cudaStream_t stream) {
+                                    int n_splits, int pages, float* parts, long long part_floats, int* error_flag, cudaStream_t stream) {
   if (sb->n_seqs <= 0) return PTB_OK;
   if (!known(heads, kv_heads, dim, pool_pages) || heads / kv_heads > 128 || sb->n_tokens != sb->n_seqs || rot_pairs < 0 || 2 * rot_pairs > dim ||
-      window < 0 || !splits_known(n_splits) || error_flag == nullptr || (rot_pairs > 0 && (rope_cos == nullptr || rope_sin == nullptr)))
+      window < 0 || error_flag == nullptr || (rot_pairs > 0 && (rope_cos == nullptr || rope_sin == nullptr)))
     return PTB_ERR_SIZE;
   if (!aligned16(fused) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
-  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, heads / kv_heads, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
+  const int rows = heads / kv_heads;
+  const Plan q = plan_of(dim, rows);
+  n_splits = splits_or(n_splits, sb->n_seqs, kv_heads, rows, 1, pages, sb->n_tokens, q);
+  if (!splits_known(n_splits)) return PTB_ERR_SIZE;
+  if (ptb_attention_q8_floats(sb->n_seqs, kv_heads, rows, 1, dim, n_splits, pages, sb->n_tokens) > part_floats) return PTB_NEEDS_WORKSPACE;
   AttnQ8 p = {};
   p.rows = (const __nv_bfloat16*)fused; p.k_pool = (uint8_t*)k_pool; p.v_pool = (uint8_t*)v_pool; p.k_exp = (int8_t*)k_exp;
   p.v_exp = (int8_t*)v_exp; p.out = (__nv_bfloat16*)out; p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.slopes = slopes;
   p.heads = heads; p.kv_heads = kv_heads; p.dim = dim; p.pool_pages = pool_pages; p.rot_pairs = rot_pairs; p.interleaved = interleaved;
   p.write_cache = write_cache; p.window = window; p.n_splits = n_splits; p.scale = scale; p.parts = parts; p.error_flag = error_flag;
-  const Plan q = plan_of(dim, heads / kv_heads);
   p.row_groups = q.row_groups; p.page_parts = q.page_parts; p.rings = q.rings; p.stages = q.stages;
   p.teams = teams_of(n_splits); p.cluster = n_splits / p.teams;
   return launch_any<true>(*sb, p, q, dim3(sb->n_seqs, kv_heads, n_splits), stream);
@@ -947,18 +949,19 @@ PTB_API int ptb_attention_decode_q8(const void* fused, void* k_pool, void* k_exp
 // tile_tokens consecutive new tokens of one sequence.
 PTB_API int ptb_attention_q8(const void* q_rows, const void* k_pool, const void* k_exp, const void* v_pool, const void* v_exp, int pool_pages,
                              void* out, const StepBatch* sb, const int* tile_seq, const int* tile_q0, int n_tiles, int tile_tokens,
-                             const float* slopes, int heads, int kv_heads, int dim, float scale, int window, int n_splits, float* parts,
+                             const float* slopes, int heads, int kv_heads, int dim, float scale, int window, int n_splits, int pages, float* parts,
                              long long part_floats, int* error_flag, cudaStream_t stream) {
   if (n_tiles <= 0) return PTB_OK;
-  if (!known(heads, kv_heads, dim, pool_pages) || window < 0 || !splits_known(n_splits) || error_flag == nullptr || tile_tokens < 1 ||
+  if (!known(heads, kv_heads, dim, pool_pages) || window < 0 || error_flag == nullptr || tile_tokens < 1 ||
       (long long)tile_tokens * (heads / kv_heads) > (1 << 24))
     return PTB_ERR_SIZE;
   if (!aligned16(q_rows) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) || (reinterpret_cast<uintptr_t>(parts) & 15)) return PTB_ERR_ALIGN;
   const int rows = tile_tokens * (heads / kv_heads);
-  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, dim, n_splits) > part_floats) return PTB_ERR_SIZE;
   const Plan q = plan_of(dim, rows);
+  n_splits = splits_or(n_splits, n_tiles, kv_heads, rows, tile_tokens, pages, sb->n_tokens, q);
   const long long chunks = (rows + q.rows_pad - 1) / q.rows_pad;
-  if (chunks * kv_heads > 65535) return PTB_ERR_SIZE;
+  if (!splits_known(n_splits) || chunks * kv_heads > 65535) return PTB_ERR_SIZE;
+  if (ptb_attention_q8_floats(n_tiles, kv_heads, rows, tile_tokens, dim, n_splits, pages, sb->n_tokens) > part_floats) return PTB_NEEDS_WORKSPACE;
   AttnQ8 p = {};
   p.rows = (const __nv_bfloat16*)q_rows; p.k_pool = (uint8_t*)k_pool; p.v_pool = (uint8_t*)v_pool; p.k_exp = (int8_t*)k_exp;
   p.v_exp = (int8_t*)v_exp; p.out = (__nv_bfloat16*)out; p.slopes = slopes; p.tile_seq = tile_seq; p.tile_q0 = tile_q0;

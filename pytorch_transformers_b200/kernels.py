@@ -7,8 +7,8 @@ calls fail.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -120,7 +120,7 @@ def lib():
                      "ptb_head_norm_gate_act", "ptb_gla_decay", "ptb_gla_walk", "ptb_gla_chunks", "ptb_gla_max_dim",
                      "ptb_gla_chunk_tokens", "ptb_delta_prepare", "ptb_delta_walk", "ptb_delta_chunks",
                      "ptb_delta_chunks_supports", "ptb_post_norm", "ptb_token_gate", "ptb_round_rows", "ptb_route_biased", "ptb_attention_tc_sizes", "ptb_attention_tc_supports_sizes", "ptb_attention_tc_extras",
-                     "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_q8_splits", "ptb_attention_decode_q8", "ptb_attention_q8",
+                     "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_decode_q8", "ptb_attention_q8",
                      "ptb_attention_tc_extras_biased", "ptb_pitch_rows"):
             getattr(L, name).restype = ctypes.c_int
         L.ptb_latent_part_floats.restype = ctypes.c_longlong
@@ -132,12 +132,11 @@ def lib():
         P, I, N, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
         L.ptb_store_q8.argtypes = [P] * 6 + [I, P, P, P] + [I] * 5 + [P, P]
         L.ptb_unpack_q8.argtypes = [P] * 4 + [I, P, P, P, I, I, P, P, I, I, I, P, P]
-        L.ptb_attention_q8_splits.argtypes = [I] * 5
-        L.ptb_attention_q8_floats.argtypes = [I] * 5
+        L.ptb_attention_q8_floats.argtypes = [I] * 8
         L.ptb_pitch_rows.argtypes = [P, P, N, I, I, P]
         L.ptb_attention_tc_extras_biased.argtypes = [P] * 3 + [I, P, P, P, P, I, P, I, I, I, F, I, P, P]
-        L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, P, N, P, P]
-        L.ptb_attention_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, P, N, P, P]
+        L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, I, P, N, P, P]
+        L.ptb_attention_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, P, N, P, P]
         L.ptb_copy_pages.argtypes = [P] * 6 + [I, P, P, N, I, I, P]
         _configured = True
     return L
@@ -1803,18 +1802,39 @@ def round_rows(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 # K/V head; a value is code * 2^exponent. csrc/q8.cuh says why a power of two.
 Q8 = torch.float8_e4m3fn
 Q8_MAX_HEADS = 128       # query heads a K/V head in attention_decode_q8
+_NEEDS_WORKSPACE = -1    # of attention_decode_q8 and attention_q8: nothing was launched
 
 
 def q8_supports(head_dim: int) -> bool:
     return 16 <= head_dim <= 256 and head_dim % 16 == 0
 
 
-_NO_GUARD = contextlib.nullcontext()
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _on_device(t: torch.Tensor):
-    """The device guard of ``t``'s device where it is not the current one (a launch goes to a stream of the current device)."""
-    return _NO_GUARD if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+def _on_its_device(function):
+    """For faces whose first argument is a tensor, or a sequence of them: called with its device as the current one, since a
+    launch goes to a stream of the current device."""
+    @functools.wraps(function)
+    def call(first, *args, **kwargs):
+        t = first if isinstance(first, torch.Tensor) else first[0]
+        device = t.get_device()
+        if device < 0 or device == _current_device():      # host memory: the face refuses it
+            return function(first, *args, **kwargs)
+        with torch.cuda.device(device):
+            return function(first, *args, **kwargs)
+    return call
+
+
+def _flag_at(device: int) -> int:
+    """Address of ``error_flag`` of the device with this number."""
+    at = _flag_addresses.get(device)
+    if at is None:
+        at = _flag_addresses[device] = error_flag(torch.device("cuda", device)).data_ptr()
+    return at
+
+
+_flag_addresses = {}
 
 
 def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Tensor, seq_new: torch.Tensor, seq_past: torch.Tensor,
@@ -1874,6 +1894,7 @@ def _check_slopes(slopes, heads: int, device: int, what: str):
     return slopes.data_ptr()
 
 
+@_on_its_device
 def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
                           batch: StepBatchC, kv_heads: int, q_per_kv: int, head_dim: int, write_cache: bool = True, rope=None,
                           interleaved: bool = False) -> torch.Tensor:
@@ -1883,31 +1904,33 @@ def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torc
     codes are then rounded again. What is infinite or no number is held as no number. bfloat16."""
     what = "split_rotate_store_q8"
     cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
-    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, fused.get_device(), what)
+    device = fused.get_device()
+    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     q = fused.new_empty((fused.shape[0], kv_heads * q_per_kv, head_dim))
     cache = (k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr()) if write_cache else (None,) * 4
-    with _on_device(fused):
-        _check(lib().ptb_store_q8(fused.data_ptr(), q.data_ptr(), *cache, pages, ctypes.byref(batch), cos, sin, pairs, interleaved,
-                                  kv_heads, q_per_kv, head_dim, error_flag(fused.device).data_ptr(), _stream(fused)), what)
+    _check(lib().ptb_store_q8(fused.data_ptr(), q.data_ptr(), *cache, pages, ctypes.byref(batch), cos, sin, pairs, interleaved, kv_heads,
+                              q_per_kv, head_dim, _flag_at(device), _raw_stream(device)), what)
     return q
 
 
+@_on_its_device
 def unpack_pages_q8(k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor, ids: torch.Tensor):
     """The pages that ``ids`` (int32, on the device) names as bfloat16 values, keys and values: [len(ids), kv_heads, PAGE, head_dim]
     each. A page out of range reads as zeros and raises the device's error flag."""
     if not (ids.dtype is torch.int32 and ids.dim() == 1 and ids.is_contiguous() and ids.is_cuda and k_pool.dim() == 4):
         raise KernelError("unpack_pages_q8 takes pages of one cache entry and a contiguous int32 list of page numbers on the device")
     _, kv_heads, _, head_dim = k_pool.shape
-    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, ids.get_device(), "unpack_pages_q8")
-    n = ids.numel()
-    k, v = (torch.empty((n, kv_heads, PAGE, head_dim), dtype=torch.bfloat16, device=ids.device) for _ in range(2))
-    with _on_device(ids):
-        _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pages, ids.data_ptr(), None,
-                                   None, n, 0, k.data_ptr(), v.data_ptr(), kv_heads, head_dim, head_dim,
-                                   error_flag(ids.device).data_ptr(), _stream(ids)), "unpack_pages_q8")
+    device, n = ids.get_device(), ids.numel()
+    pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, "unpack_pages_q8")
+    shape = (n, kv_heads, PAGE, head_dim)
+    k, v = ids.new_empty(shape, dtype=torch.bfloat16), ids.new_empty(shape, dtype=torch.bfloat16)
+    _check(lib().ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pages, ids.data_ptr(), None, None, n,
+                               0, k.data_ptr(), v.data_ptr(), kv_heads, head_dim, head_dim, _flag_at(device), _raw_stream(device)),
+           "unpack_pages_q8")
     return k, v
 
 
+@_on_its_device
 def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
                         batch: StepBatchC, rope, slopes: Optional[torch.Tensor], kv_heads: int, q_per_kv: int, head_dim: int,
                         scale: float, window: int = 0, write_cache: bool = True, interleaved: bool = False, n_splits: int = 0,
@@ -1925,29 +1948,26 @@ def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.
     n = batch.n_seqs
     if batch.n_tokens != n or q_per_kv > Q8_MAX_HEADS or window < 0 or n_splits < 0:
         raise KernelError(f"{what} takes one token a sequence and at most {Q8_MAX_HEADS} query heads a K/V head")
+    if n_splits > 8:
+        n_splits = n_splits // 8 * 8
+    pages = max_pages or batch.pages_stride
+    if window:
+        pages = min(pages, window // PAGE + 2)
     L = lib()
-    parts = parts_at = None
-    floats = 0
-    with _on_device(fused):
-        if n_splits == 0:
-            pages = max_pages or batch.pages_stride
-            if window:
-                pages = min(pages, window // PAGE + 2)
-            n_splits = L.ptb_attention_q8_splits(n, kv_heads, q_per_kv, head_dim, pages)
-        elif n_splits > 8:
-            n_splits = n_splits // 8 * 8
-        if n_splits > 8:
-            floats = L.ptb_attention_q8_floats(n, kv_heads, q_per_kv, head_dim, n_splits)
-            parts = torch.empty(floats, dtype=torch.float32, device=fused.device)
-            parts_at = parts.data_ptr()
-        out = fused.new_empty((n, heads * head_dim))
-        _check(L.ptb_attention_decode_q8(fused.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(),
-                                         pool_pages, out.data_ptr(), ctypes.byref(batch), cos, sin, pairs, interleaved, slopes_at,
-                                         heads, kv_heads, head_dim, scale, window, write_cache, n_splits, parts_at, floats,
-                                         error_flag(fused.device).data_ptr(), _stream(fused)), what)
+    out = fused.new_empty((n, heads * head_dim))
+    args = (fused.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pool_pages, out.data_ptr(),
+            ctypes.byref(batch), cos, sin, pairs, interleaved, slopes_at, heads, kv_heads, head_dim, scale, window, write_cache, n_splits, pages)
+    flag, stream = _flag_at(device), _raw_stream(device)
+    code = L.ptb_attention_decode_q8(*args, None, 0, flag, stream)
+    if code == _NEEDS_WORKSPACE:      # more than a cluster of blocks for a row: they join through memory
+        floats = L.ptb_attention_q8_floats(n, kv_heads, q_per_kv, 1, head_dim, n_splits, pages, n)
+        parts = torch.empty(floats, dtype=torch.float32, device=fused.device)
+        code = L.ptb_attention_decode_q8(*args, parts.data_ptr(), floats, flag, stream)
+    _check(code, what)
     return out
 
 
+@_on_its_device
 def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
                  batch: StepBatchC, tile_seq: torch.Tensor, tile_q0: torch.Tensor, n_tiles: int, tile_tokens: int,
                  slopes: Optional[torch.Tensor], kv_heads: int, scale: float, window: int = 0, n_pages: int = 0,
@@ -1969,28 +1989,25 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     for t in (tile_seq, tile_q0):
         if not (t.dtype is torch.int32 and t.numel() >= n_tiles and t.get_device() == device and t.is_contiguous()):
             raise KernelError(f"{what}: tile lists must be contiguous int32 tensors of {n_tiles} tiles on the queries' device")
-    L = lib()
     if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and head_dim <= 128:
         return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
                                       window, n_pages)
-    rows = tile_tokens * (heads // kv_heads)
-    parts = parts_at = None
-    floats = 0
-    with _on_device(q):
-        if n_splits == 0:
-            pages = batch.pages_stride if n_pages <= 0 else min(batch.pages_stride, n_pages)
-            n_splits = L.ptb_attention_q8_splits(n_tiles, kv_heads, rows, head_dim, pages)
-        elif n_splits > 8:
-            n_splits = n_splits // 8 * 8
-        if n_splits > 8:
-            floats = L.ptb_attention_q8_floats(n_tiles, kv_heads, rows, head_dim, n_splits)
-            parts = torch.empty(floats, dtype=torch.float32, device=q.device)
-            parts_at = parts.data_ptr()
-        out = q.new_empty((n, heads * head_dim))
-        _check(L.ptb_attention_q8(q.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pool_pages,
-                                  out.data_ptr(), ctypes.byref(batch), tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, tile_tokens,
-                                  slopes_at, heads, kv_heads, head_dim, scale, window, n_splits, parts_at, floats,
-                                  error_flag(q.device).data_ptr(), _stream(q)), what)
+    if n_splits > 8:
+        n_splits = n_splits // 8 * 8
+    pages = batch.pages_stride if n_pages <= 0 else min(batch.pages_stride, n_pages)
+    L = lib()
+    out = q.new_empty((n, heads * head_dim))
+    args = (q.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pool_pages, out.data_ptr(),
+            ctypes.byref(batch), tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, tile_tokens, slopes_at, heads, kv_heads, head_dim,
+            scale, window, n_splits, pages)
+    flag, stream = _flag_at(device), _raw_stream(device)
+    code = L.ptb_attention_q8(*args, None, 0, flag, stream)
+    if code == _NEEDS_WORKSPACE:
+        floats = L.ptb_attention_q8_floats(n_tiles, kv_heads, tile_tokens * (heads // kv_heads), tile_tokens, head_dim, n_splits,
+                                           pages, n)
+        parts = torch.empty(floats, dtype=torch.float32, device=q.device)
+        code = L.ptb_attention_q8(*args, parts.data_ptr(), floats, flag, stream)
+    _check(code, what)
     return out
 
 
@@ -2002,27 +2019,25 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
     room = (n_pages + step - 1) // step * step
     k, v = (torch.empty((room, kv_heads, PAGE, wide), dtype=torch.bfloat16, device=device) for _ in range(2))
     table = torch.empty((batch.n_seqs, batch.pages_stride), dtype=torch.int32, device=device)
-    L, flag = lib(), error_flag(device).data_ptr()
-    with _on_device(q):
-        stream = _stream(q)
-        _check(L.ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
-                               ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
-                               wide, flag, stream), "attention_q8 (pages)")
-        unpacked = StepBatchC.from_buffer_copy(batch)
-        unpacked.pages = table.data_ptr()
-        if wide != head_dim:
-            own, q = q, q.new_empty((n, heads, wide))
-            _check(L.ptb_pitch_rows(own.data_ptr(), q.data_ptr(), n * heads, head_dim, wide, stream), "attention_q8 (queries)")
-        if slopes is None:
-            out = attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
-        else:
-            out = q.new_empty((n, heads * wide))
-            _check(L.ptb_attention_tc_extras_biased(q.data_ptr(), k.data_ptr(), v.data_ptr(), room, out.data_ptr(), ctypes.byref(unpacked),
-                                                    tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, slopes.data_ptr(), heads, kv_heads,
-                                                    wide, scale, window, flag, stream), "attention_q8 (prompt)")
-        if wide != head_dim:
-            padded, out = out, q.new_empty((n, heads * head_dim))
-            _check(L.ptb_pitch_rows(padded.data_ptr(), out.data_ptr(), n * heads, wide, head_dim, stream), "attention_q8 (result)")
+    L, flag, stream = lib(), _flag_at(device.index), _raw_stream(device.index)
+    _check(L.ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
+                           ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
+                           wide, flag, stream), "attention_q8 (pages)")
+    unpacked = StepBatchC.from_buffer_copy(batch)
+    unpacked.pages = table.data_ptr()
+    if wide != head_dim:
+        own, q = q, q.new_empty((n, heads, wide))
+        _check(L.ptb_pitch_rows(own.data_ptr(), q.data_ptr(), n * heads, head_dim, wide, stream), "attention_q8 (queries)")
+    if slopes is None:
+        out = attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
+    else:
+        out = q.new_empty((n, heads * wide))
+        _check(L.ptb_attention_tc_extras_biased(q.data_ptr(), k.data_ptr(), v.data_ptr(), room, out.data_ptr(), ctypes.byref(unpacked),
+                                                tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, slopes.data_ptr(), heads, kv_heads,
+                                                wide, scale, window, flag, stream), "attention_q8 (prompt)")
+    if wide != head_dim:
+        padded, out = out, q.new_empty((n, heads * head_dim))
+        _check(L.ptb_pitch_rows(padded.data_ptr(), out.data_ptr(), n * heads, wide, head_dim, stream), "attention_q8 (result)")
     return out
 
 
@@ -2056,8 +2071,10 @@ def copy_pages(pools, src, dst, out=None):
                                for q, m, e in zip(to_at, to_step, entries) if n * f and m * e):
         raise KernelError("copy_pages: the targets lie in the sources' memory")
     pointers, numbers = ctypes.c_void_p * k, ctypes.c_longlong * k
-    with _on_device(t):
-        _check(lib().ptb_copy_pages(pointers(*from_at), pointers(*to_at), numbers(*from_step), numbers(*to_step), numbers(*page_bytes),
-                                    (ctypes.c_int * k)(*entries), k, src.ctypes.data, dst.ctypes.data, src.size, n_src, n_dst,
-                                    _stream(t)), "copy_pages")
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return copy_pages(pools, src, dst, out=out)
+    _check(lib().ptb_copy_pages(pointers(*from_at), pointers(*to_at), numbers(*from_step), numbers(*to_step), numbers(*page_bytes),
+                                (ctypes.c_int * k)(*entries), k, src.ctypes.data, dst.ctypes.data, src.size, n_src, n_dst,
+                                _raw_stream(device)), "copy_pages")
     return into
