@@ -105,94 +105,6 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(h) : "f"(hi), "f"(lo));
   return h;
 }
-// Eighths of rows of the projection on their way (a row's own and the one that holds its pairs' other halves), and the angles of an
-// eighth, which are the same for all rows: what a lane rotates in registers once all of its loads are out.
-struct Angles {
-  float c[8], s[8];
-  int mode;      // 0: not rotated; 1: pairs within the eighth; 2: the pairs' other halves in the eighth `other`; 3: entry by entry
-  int other;
-  bool upper;
-};
-__device__ __forceinline__ Angles angles_of(int c, const float* rc, const float* rs, int P, int interleaved) {
-  Angles a;
-  const int d0 = 8 * c;
-  a.other = c;
-  a.upper = d0 >= P;
-  a.mode = d0 >= 2 * P ? 0 : interleaved ? 1 : (P & 7) == 0 ? 2 : 3;
-  if (a.mode == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (d0 / 2 + i < P) a.c[i] = rc[d0 / 2 + i], a.s[i] = rs[d0 / 2 + i];
-      else a.c[i] = 1.f, a.s[i] = 0.f;
-  } else if (a.mode == 2) {
-    const int e0 = a.upper ? d0 - P : d0;
-    a.other = (a.upper ? e0 : e0 + P) / 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a.c[i] = rc[e0 + i], a.s[i] = rs[e0 + i];
-  }
-  return a;
-}
-__device__ __forceinline__ void rotate8(const Angles& a, const uint4& own, const uint4& other, float (&x)[8]) {
-  unpack_bf16x8(own, x);
-  if (a.mode == 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (a.c[i] != 1.f || a.s[i] != 0.f) rotate_pair(x[2 * i], x[2 * i + 1], a.c[i], a.s[i], x[2 * i], x[2 * i + 1]);
-  } else if (a.mode == 2) {
-    float y[8];
-    unpack_bf16x8(other, y);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float ra, rb;
-      rotate_pair(a.upper ? y[i] : x[i], a.upper ? x[i] : y[i], a.c[i], a.s[i], ra, rb);
-      x[i] = a.upper ? rb : ra;
-    }
-  }
-}
-
-// One token's key (or value) into its page, by one warp: the rule of store_q8_kernel for a page that gets one row. The row's codes go to
-// `copy` as well, and the page's exponent is returned; `rose`: it is larger than before, and the earlier codes have been
-// rounded again, seen by all who read them after the block's next barrier.
-__device__ int append_row(const __nv_bfloat16* row, const float* rc, const float* rs, int P, int interleaved, uint8_t* codes, int8_t* exps,
-                          int at, int dim, unsigned char* copy, bool& rose) {
-  const int lane = threadIdx.x & 31;
-  const int old = at > 0 ? int(__ldcg(reinterpret_cast<const signed char*>(exps))) : Q8_EXP_MIN;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, most = 0.f;
-  if (lane * 8 < dim) {
-    load_rotated8(row, lane, rc, rs, P, interleaved, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, finite_abs(x[e]));
-  }
-  const int e = max(q8_exponent(warp_max(most)), old);
-  rose = at > 0 && e > old;
-  if (rose) {
-    const float down = power_of_two(max(old - e, -126));
-    for (int i = lane; i < at * dim / 16; i += 32) {
-      uint4 w = __ldcg(reinterpret_cast<const uint4*>(codes) + i);
-      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float f[4];
-        q8_unpack4(u[k], f);
-        u[k] = q8_pack4(f[0] * down, f[1] * down, f[2] * down, f[3] * down);
-      }
-      reinterpret_cast<uint4*>(codes)[i] = w;
-    }
-  }
-  const float by = power_of_two(-e);
-  if (lane * 8 < dim) {
-    const uint2 w = make_uint2(q8_pack4(x[0] * by, x[1] * by, x[2] * by, x[3] * by), q8_pack4(x[4] * by, x[5] * by, x[6] * by, x[7] * by));
-    *reinterpret_cast<uint2*>(codes + size_t(at) * dim + lane * 8) = w;
-    *reinterpret_cast<uint2*>(copy + lane * 8) = w;
-  }
-  if (lane == 0) *exps = int8_t(e);
-  if (rose) {      // the accelerator reads them next
-    __threadfence();
-    asm volatile("fence.proxy.async;\n" ::: "memory");
-  }
-  return e;
-}
-
 template <int DP, int NH, bool FUSED>
 __global__ void __launch_bounds__(WARPS * 32, Q8Shape<DP, NH>::BLOCKS)
 attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
@@ -236,6 +148,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   const int n_rows = min(rows_pad, tokens * qpk - row0);
   if (n_rows <= 0) return;      // all blocks of a cluster alike
   const int past = sb.seq_past[seq], start = sb.seq_start[seq];
+  if (FUSED && sb.seq_new[seq] != 1 && tid == 0) atomicExch(p.error_flag, 24);
   const int first_pos = FUSED ? past : past + q0 + row0 / qpk, last_pos = FUSED ? past : past + q0 + (row0 + n_rows - 1) / qpk;
   const int low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;      // the first key that a row sees
   const int* pages = sb.pages + size_t(seq) * sb.pages_stride;

@@ -5,15 +5,15 @@
 
 namespace {
 
-constexpr int STORE_THREADS = 256;
+constexpr int STORE_THREADS = 256, Q_HEADS = 4;
 
 // ------------------------------------------------------------------------------------------------ append
 // Projection rows into rotated queries, and keys (rotated) and values into the pages.
 //
 // The first blocks take a page each: (page that the step writes to) x (K/V head) x (keys or values). A page's new rows, 64 at most,
 // stay in registers between the reduction that gives its exponent and the rounding: one pass over the projection. One block
-// has the page to itself, so no order among blocks can change what a page holds. The other blocks rotate queries, a
-// thread eight entries at a time.
+// has the page to itself, so no order among blocks can change what a page holds. The other blocks rotate queries: a thread has an eighth of a
+// head (with pairs (i, i + n) that eighth and its pairs' other halves) of up to four heads of a token, whose angles are the same.
 struct StoreParams {
   const __nv_bfloat16* fused;
   __nv_bfloat16* q_out;
@@ -22,6 +22,7 @@ struct StoreParams {
   const float *rope_cos, *rope_sin;
   int rot_pairs, interleaved, kv_heads, q_per_kv, dim, pool_pages;
   int page_blocks;             // blocks of pages; the others are queries'
+  int halves, q_units;         // pairs (i, i + n) in whole eighths; threads for a head
   int* error_flag;
 };
 
@@ -32,18 +33,63 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
   const int tid = threadIdx.x, eighths = p.dim / 8, rows = p.q_per_kv + 2;
   const size_t width = size_t(p.kv_heads) * rows * p.dim;
   if (int(blockIdx.x) >= p.page_blocks) {
-    const int heads = p.kv_heads * p.q_per_kv;
-    const long long total = (long long)sb.n_tokens * heads * eighths;
+    const int heads = p.kv_heads * p.q_per_kv, groups = (heads + Q_HEADS - 1) / Q_HEADS;
     const long long i = (long long)(blockIdx.x - p.page_blocks) * STORE_THREADS + tid;
-    if (i >= total) return;
-    const int c = int(i % eighths);
-    const long long th = i / eighths;
-    const int h = int(th % heads), t = int(th / heads);
-    const int g = h / p.q_per_kv;
-    const __nv_bfloat16* row = p.fused + size_t(t) * width + size_t(g * rows + h - g * p.q_per_kv) * p.dim;
-    float x[8];
-    load_rotated8(row, c, p.rope_cos + size_t(t) * p.rot_pairs, p.rope_sin + size_t(t) * p.rot_pairs, p.rot_pairs, p.interleaved, x);
-    *reinterpret_cast<uint4*>(p.q_out + (size_t(th) * eighths + c) * 8) = pack_bf16x8(x);
+    if (i >= (long long)sb.n_tokens * groups * p.q_units) return;
+    const int at = int(i / p.q_units), unit = int(i - (long long)at * p.q_units), t = at / groups, h0 = (at - t * groups) * Q_HEADS;
+    const float *rc = p.rope_cos + size_t(t) * p.rot_pairs, *rs = p.rope_sin + size_t(t) * p.rot_pairs;
+    const uint4* row = reinterpret_cast<const uint4*>(p.fused + size_t(t) * width);
+    uint4* out = reinterpret_cast<uint4*>(p.q_out + size_t(t) * heads * p.dim);
+    const int half = p.rot_pairs / 8;
+    const bool both = p.halves && unit < half;      // eighth `unit` and the one of its pairs' other halves
+    const int c = p.halves && !both ? unit + half : unit;
+    uint4 own[Q_HEADS], other[Q_HEADS];
+#pragma unroll
+    for (int k = 0; k < Q_HEADS; ++k) {
+      const int h = min(h0 + k, heads - 1), g = h / p.q_per_kv;
+      const uint4* head = row + (g * rows + h - g * p.q_per_kv) * eighths;
+      own[k] = head[c];
+      other[k] = both ? head[c + half] : own[k];
+    }
+    if (both) {
+      float cs[8], sn[8];
+      load_angles(rc, rs, 8 * unit, cs, sn);
+#pragma unroll
+      for (int k = 0; k < Q_HEADS; ++k) {
+        if (h0 + k >= heads) break;
+        float x[8], y[8];
+        rotate_halves(cs, sn, own[k], other[k], x, y);
+        out[(h0 + k) * eighths + c] = pack_bf16x8(x);
+        out[(h0 + k) * eighths + c + half] = pack_bf16x8(y);
+      }
+      return;
+    }
+    const Angles angles = angles_of(c, rc, rs, p.halves ? 0 : p.rot_pairs, p.interleaved);      // past the rotated entries, or other kinds of pairs
+#pragma unroll
+    for (int k = 0; k < Q_HEADS; ++k) {
+      if (h0 + k >= heads) break;
+      const int h = h0 + k, g = h / p.q_per_kv;
+      float x[8];
+      if (angles.mode == 3) load_rotated8(reinterpret_cast<const __nv_bfloat16*>(row + (g * rows + h - g * p.q_per_kv) * eighths), c, rc, rs, p.rot_pairs, 0, x);
+      else rotate8(angles, own[k], own[k], x);
+      out[h * eighths + c] = pack_bf16x8(x);
+    }
+    return;
+  }
+  if (sb.n_tokens == sb.n_seqs) {      // single tokens: a warp for a row (64 sequences, 8 K/V heads: 3.1 us; a block for each 8.5)
+    const int at = blockIdx.x * (STORE_THREADS / 32) + tid / 32, seq = at / (2 * p.kv_heads), g = at % (2 * p.kv_heads) >> 1;
+    if (seq >= sb.n_seqs) return;
+    const bool keys = (at & 1) == 0;
+    const int past = sb.seq_past[seq], page = sb.pages[size_t(seq) * sb.pages_stride + past / PTB_PAGE];
+    if (page < 0 || page >= p.pool_pages || sb.seq_new[seq] != 1) {      // 24: as many tokens as sequences, but not one each
+      if ((tid & 31) == 0) atomicExch(p.error_flag, sb.seq_new[seq] != 1 ? 24 : 21);
+      return;
+    }
+    const size_t block = size_t(page) * p.kv_heads + g, t = sb.seq_start[seq];
+    bool rose;
+    append_row(p.fused + t * width + size_t(g * rows + p.q_per_kv + (keys ? 0 : 1)) * p.dim, p.rope_cos + t * p.rot_pairs, p.rope_sin + t * p.rot_pairs,
+               keys ? p.rot_pairs : 0, p.interleaved, (keys ? p.k_pool : p.v_pool) + block * PTB_PAGE * p.dim, (keys ? p.k_exp : p.v_exp) + block,
+               past % PTB_PAGE, p.dim, nullptr, rose);
     return;
   }
   const int job = blockIdx.x / (2 * p.kv_heads), rest = blockIdx.x % (2 * p.kv_heads);
@@ -69,9 +115,27 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
   int8_t* exps = (keys ? p.k_exp : p.v_exp) + block;
   const int old = *exps;
   const __nv_bfloat16* src = p.fused + size_t(g * rows + p.q_per_kv + (keys ? 0 : 1)) * p.dim;
-  const int total = (last - first) * eighths;
+  // keys whose every entry is rotated, in halves: a thread takes an eighth and that of its pairs' other halves, x[k] and x[k + MOST / 2]
+  const bool both = keys && p.halves && 2 * p.rot_pairs == p.dim;
+  const int half = p.rot_pairs / 8, total = (last - first) * (both ? half : eighths);
   float x[MOST][8];
   float most = 0.f;
+  if (both) {
+#pragma unroll
+    for (int k = 0; k < MOST / 2; ++k) {
+      const int i = tid + k * STORE_THREADS;
+      if (i < total) {
+        const int r = i / half, c = i - r * half;
+        const size_t t = t0 + r;
+        const uint4* row = reinterpret_cast<const uint4*>(src + t * width);
+        float cs[8], sn[8];
+        load_angles(p.rope_cos + t * p.rot_pairs, p.rope_sin + t * p.rot_pairs, 8 * c, cs, sn);
+        rotate_halves(cs, sn, row[c], row[c + half], x[k], x[k + MOST / 2]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fmaxf(finite_abs(x[k][e]), finite_abs(x[k + MOST / 2][e])));
+      }
+    }
+  } else
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     const int i = tid + k * STORE_THREADS;
@@ -102,13 +166,26 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
     }
   }
   const float by = power_of_two(-e);
+  auto codes8 = [&](const float (&v)[8]) {
+    return make_uint2(q8_pack4(v[0] * by, v[1] * by, v[2] * by, v[3] * by), q8_pack4(v[4] * by, v[5] * by, v[6] * by, v[7] * by));
+  };
+  if (both) {
+#pragma unroll
+    for (int k = 0; k < MOST / 2; ++k) {
+      const int i = tid + k * STORE_THREADS;
+      if (i < total) {
+        const int r = i / half, c = i - r * half;
+        uint2* to = reinterpret_cast<uint2*>(codes + size_t(first + r) * p.dim) + c;
+        to[0] = codes8(x[k]);
+        to[half] = codes8(x[k + MOST / 2]);
+      }
+    }
+  } else
 #pragma unroll
   for (int k = 0; k < MOST; ++k) {
     const int i = tid + k * STORE_THREADS;
     if (i < total) {
-      const uint2 w = make_uint2(q8_pack4(x[k][0] * by, x[k][1] * by, x[k][2] * by, x[k][3] * by),
-                                 q8_pack4(x[k][4] * by, x[k][5] * by, x[k][6] * by, x[k][7] * by));
-      *reinterpret_cast<uint2*>(codes + size_t(first) * p.dim + size_t(i) * 8) = w;      // rows of a page lie one after another
+      *reinterpret_cast<uint2*>(codes + size_t(first) * p.dim + size_t(i) * 8) = codes8(x[k]);      // rows of a page lie one after another
     }
   }
   if (tid == 0) *exps = int8_t(e);      // every thread has read the old one: the reduction lies between
@@ -212,16 +289,35 @@ __device__ __forceinline__ void copy_units(const CopyParams& p, const CopyTensor
   const long long base = block * (COPY_THREADS * COPY_ILP) + threadIdx.x;
   W w[COPY_ILP];
   W* to[COPY_ILP];
+  // One division for the first unit (in 32 bits where they do): its 64-bit form for each unit was most of the kernel's time. The
+  // others lie COPY_THREADS apart, in the same page or a next one.
+  const bool narrow = t.units < (1ll << 32);
+  long long page = narrow ? (long long)(unsigned(base) / unsigned(per_page)) : base / per_page;
+  long long in = base - page * per_page;
+  const W* from = nullptr;
+  W* into = nullptr;
 #pragma unroll
   for (int k = 0; k < COPY_ILP; ++k) {
     const long long u = base + k * COPY_THREADS;
+    if (k > 0) {
+      in += COPY_THREADS;
+      if (in >= per_page) {
+        const long long on = per_page >= COPY_THREADS ? 1 : narrow ? (long long)(unsigned(in) / unsigned(per_page)) : in / per_page;
+        page += on;
+        in -= on * per_page;
+        from = nullptr;
+      }
+    }
     to[k] = nullptr;
     if (u < t.units) {
-      const long long page = u / per_page, in = u - page * per_page;
-      const int pair = int(page % p.n_pairs);
-      const long long entry = page / p.n_pairs;
-      w[k] = *(reinterpret_cast<const W*>(t.src + entry * t.src_entry + p.src[pair] * t.page_bytes) + in);
-      to[k] = reinterpret_cast<W*>(t.dst + entry * t.dst_entry + p.dst[pair] * t.page_bytes) + in;
+      if (from == nullptr) {
+        const unsigned entry = unsigned(page) / unsigned(p.n_pairs);      // pages: pairs * entries, below 2^31
+        const int pair = int(unsigned(page) - entry * unsigned(p.n_pairs));
+        from = reinterpret_cast<const W*>(t.src + (long long)entry * t.src_entry + p.src[pair] * t.page_bytes);
+        into = reinterpret_cast<W*>(t.dst + (long long)entry * t.dst_entry + p.dst[pair] * t.page_bytes);
+      }
+      w[k] = from[in];
+      to[k] = into + in;
     }
   }
 #pragma unroll
@@ -261,14 +357,18 @@ PTB_API int ptb_store_q8(const void* fused, void* q_out, void* k_pool, void* k_e
   if (!aligned16(fused) || !aligned16(q_out) || !aligned16(k_pool) || !aligned16(v_pool)) return PTB_ERR_ALIGN;
   // pages that the step writes to: one for each single token, else at most this
   const long long jobs = k_pool == nullptr ? 0 : sb->n_tokens == sb->n_seqs ? sb->n_seqs : sb->n_tokens / PTB_PAGE + 2ll * sb->n_seqs;
-  const long long page_blocks = jobs * 2 * kv_heads;
-  const long long q_blocks = ((long long)sb->n_tokens * kv_heads * q_per_kv * (dim / 8) + STORE_THREADS - 1) / STORE_THREADS;
+  const long long page_blocks = sb->n_tokens == sb->n_seqs ? (jobs * 2 * kv_heads + STORE_THREADS / 32 - 1) / (STORE_THREADS / 32) : jobs * 2 * kv_heads;
+  const int halves = rot_pairs > 0 && !interleaved && rot_pairs % 8 == 0, q_units = dim / 8 - (halves ? rot_pairs / 8 : 0);
+  const long long q_groups = ((long long)kv_heads * q_per_kv + Q_HEADS - 1) / Q_HEADS;
+  if ((long long)sb->n_tokens * q_groups > 0x7fffffffll) return PTB_ERR_SIZE;
+  const long long q_blocks = ((long long)sb->n_tokens * q_groups * q_units + STORE_THREADS - 1) / STORE_THREADS;
   if (page_blocks + q_blocks > 0x7fffffffll) return PTB_ERR_SIZE;
   StoreParams p;
   p.fused = (const __nv_bfloat16*)fused; p.q_out = (__nv_bfloat16*)q_out;
   p.k_pool = (uint8_t*)k_pool; p.v_pool = (uint8_t*)v_pool; p.k_exp = (int8_t*)k_exp; p.v_exp = (int8_t*)v_exp;
   p.rope_cos = rope_cos; p.rope_sin = rope_sin; p.rot_pairs = rot_pairs; p.interleaved = interleaved;
   p.kv_heads = kv_heads; p.q_per_kv = q_per_kv; p.dim = dim; p.pool_pages = pool_pages; p.page_blocks = int(page_blocks);
+  p.halves = halves; p.q_units = q_units;
   p.error_flag = error_flag;
   const dim3 grid(unsigned(page_blocks + q_blocks)), block(STORE_THREADS);
   if (dim <= 128) launch_pdl(store_q8_kernel<4>, grid, block, 0, stream, *sb, p);
@@ -305,16 +405,16 @@ PTB_API int ptb_pitch_rows(const void* src, void* dst, long long rows, int from_
   return launch_status();
 }
 
-// src[i] -> dst[i] (host arrays) in each of n_tensors tensors: pages of page_bytes[k] bytes, entries of src_entry[k] and dst_entry[k] bytes.
-// Pages out of range, a target named twice, and a page that is source and target at once (where a tensor is copied within itself) are
-// refused before anything is launched: then every order of the copies gives the same bytes.
-PTB_API int ptb_copy_pages(const void* const* src_base, void* const* dst_base, const long long* src_entry, const long long* dst_entry,
-                           const long long* page_bytes, const int* entries, int n_tensors, const int* src, const int* dst, long long n_pairs,
-                           int src_pages, int dst_pages, cudaStream_t stream) {
+// src[i] -> dst[i] (host arrays) in each of n_tensors tensors, of which `tensors` has six numbers each: source and target, bytes from an
+// entry's pages to the next's in both, bytes of a page, entries. Pages out of range, a target named twice, and a page that is source and
+// target at once (where a tensor is copied within itself) are refused before anything is launched: then every order of the
+// copies gives the same bytes.
+PTB_API int ptb_copy_pages(const long long* tensors, int n_tensors, const int* src, const int* dst, long long n_pairs, int src_pages,
+                           int dst_pages, cudaStream_t stream) {
   if (n_pairs <= 0 || n_tensors <= 0) return PTB_OK;
   if (n_tensors > COPY_TENSORS || src_pages < 0 || dst_pages < 0) return PTB_ERR_SIZE;
   bool within = false;
-  for (int k = 0; k < n_tensors; ++k) within = within || src_base[k] == dst_base[k];
+  for (int k = 0; k < n_tensors; ++k) within = within || tensors[6 * k] == tensors[6 * k + 1];
   const size_t marks = size_t(src_pages) + size_t(dst_pages);
   unsigned char* seen = new (std::nothrow) unsigned char[marks + 1]();
   if (seen == nullptr) return PTB_ERR_SIZE;
@@ -337,13 +437,15 @@ PTB_API int ptb_copy_pages(const void* const* src_base, void* const* dst_base, c
     p.n_tensors = 0;
     long long blocks = 0;
     for (int k = 0; k < n_tensors; ++k) {
-      if (page_bytes[k] <= 0 || entries[k] <= 0) continue;
+      const long long* v = tensors + 6 * k;
+      if (v[4] <= 0 || v[5] <= 0) continue;
       CopyTensor& t = p.t[p.n_tensors++];
-      t.src = (const unsigned char*)src_base[k]; t.dst = (unsigned char*)dst_base[k];
-      t.src_entry = src_entry[k]; t.dst_entry = dst_entry[k]; t.page_bytes = page_bytes[k]; t.entries = entries[k];
+      t.src = reinterpret_cast<const unsigned char*>(v[0]); t.dst = reinterpret_cast<unsigned char*>(v[1]);
+      t.src_entry = v[2]; t.dst_entry = v[3]; t.page_bytes = v[4]; t.entries = int(v[5]);
       const unsigned long long bits = 16 | reinterpret_cast<uintptr_t>(t.src) | reinterpret_cast<uintptr_t>(t.dst) |
                                       (unsigned long long)t.page_bytes | (unsigned long long)t.src_entry | (unsigned long long)t.dst_entry;
       t.unit = int(bits & (~bits + 1));
+      if ((long long)p.n_pairs * t.entries > 0x7fffffffll) return PTB_ERR_SIZE;
       t.units = (long long)p.n_pairs * t.entries * (t.page_bytes / t.unit);
       t.first_block = blocks;
       blocks += (t.units + COPY_THREADS * COPY_ILP - 1) / (COPY_THREADS * COPY_ILP);

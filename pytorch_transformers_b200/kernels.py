@@ -137,7 +137,7 @@ def lib():
         L.ptb_attention_tc_extras_biased.argtypes = [P] * 3 + [I, P, P, P, P, I, P, I, I, I, F, I, P, P]
         L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, I, P, N, P, P]
         L.ptb_attention_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, P, N, P, P]
-        L.ptb_copy_pages.argtypes = [P] * 6 + [I, P, P, N, I, I, P]
+        L.ptb_copy_pages.argtypes = [P, I, P, P, N, I, I, P]
         _configured = True
     return L
 
@@ -535,6 +535,8 @@ def check_device_errors(device) -> None:
             flag.zero_()
             if code == 21:
                 raise KernelError("a page table or list named a page that the cache does not have: the results are void")
+            if code == 24:
+                raise KernelError("a step of as many tokens as sequences did not bring one token for each: its results are void")
             raise KernelError(f"a kernel gave up waiting inside its pipeline (code {code}): its results are void")
 
 
@@ -1901,7 +1903,8 @@ def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torc
     """``split_rotate_store`` for a cache in 8 bits: rotated queries [tokens, heads, head_dim] in bfloat16, and keys (rotated, not
     rounded in between) and values as codes. A page that gets its first token takes the exponent that its new rows need (the smallest
     e with max |x| <= 448 * 2^e); one with earlier tokens keeps its own unless the rows need a larger one, to which the earlier
-    codes are then rounded again. What is infinite or no number is held as no number. bfloat16."""
+    codes are then rounded again. What is infinite or no number is held as no number. bfloat16. Every sequence of the step brings a
+    token at least."""
     what = "split_rotate_store_q8"
     cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
     device = fused.get_device()
@@ -2052,29 +2055,23 @@ def copy_pages(pools, src, dst, out=None):
     k = len(pools)
     if not (0 < k <= 8 and len(into) == k and src.ndim == 1 and src.shape == dst.shape):
         raise KernelError("copy_pages takes one to eight tensors, as many targets and one target page for each source page")
-    t = pools[0]
-    device, n_src, n_dst = t.get_device(), t.shape[1], into[0].shape[1]
-    bases, page_bytes, entries = [], [], []
+    device, n_src, n_dst = pools[0].get_device(), pools[0].shape[1], into[0].shape[1]
+    flat = []      # for each tensor: addresses, bytes from an entry's pages to the next's, bytes of a page, entries
     for a, b in zip(pools, into):
         shape = a.shape
-        if not (len(shape) >= 2 and a.get_device() == b.get_device() == device >= 0 and a.dtype is b.dtype and a.is_contiguous()
-                and b.is_contiguous() and shape[1] == n_src and (a is b or (b.shape[0] == shape[0] and b.shape[2:] == shape[2:]
-                                                                            and b.shape[1] == n_dst))):
+        if not (len(shape) >= 2 and shape[1] == n_src and a.get_device() == device >= 0 and a.is_contiguous()
+                and (a is b or (b.shape[0] == shape[0] and b.shape[1] == n_dst and b.shape[2:] == shape[2:] and b.dtype is a.dtype
+                                and b.get_device() == device and b.is_contiguous()))):
             raise KernelError("copy_pages takes contiguous tensors [entries, pages, ...] on one CUDA device, all with the same number of "
                               "pages, and targets that differ in that number only")
-        bases.append((a.data_ptr(), b.data_ptr()))
-        page_bytes.append(a.element_size() * math.prod(shape[2:]))
-        entries.append(shape[0])
-    from_at, to_at = zip(*bases)
-    from_step, to_step = [n_src * p for p in page_bytes], [n_dst * p for p in page_bytes]
-    if out is not None and any(p < q + m * e and q < p + n * f for p, n, f in zip(from_at, from_step, entries)
-                               for q, m, e in zip(to_at, to_step, entries) if n * f and m * e):
+        page = a.nbytes // (shape[0] * n_src) if shape[0] and n_src else 0
+        flat += (a.data_ptr(), b.data_ptr(), n_src * page, n_dst * page, page, shape[0])
+    if out is not None and any(flat[i] < flat[j + 1] + flat[j + 3] * flat[j + 5] and flat[j + 1] < flat[i] + flat[i + 2] * flat[i + 5]
+                               for i in range(0, 6 * k, 6) for j in range(0, 6 * k, 6) if flat[i + 4] and flat[j + 4]):
         raise KernelError("copy_pages: the targets lie in the sources' memory")
-    pointers, numbers = ctypes.c_void_p * k, ctypes.c_longlong * k
     if device != _current_device():
         with torch.cuda.device(device):
             return copy_pages(pools, src, dst, out=out)
-    _check(lib().ptb_copy_pages(pointers(*from_at), pointers(*to_at), numbers(*from_step), numbers(*to_step), numbers(*page_bytes),
-                                (ctypes.c_int * k)(*entries), k, src.ctypes.data, dst.ctypes.data, src.size, n_src, n_dst,
+    _check(lib().ptb_copy_pages((ctypes.c_longlong * (6 * k))(*flat), k, src.ctypes.data, dst.ctypes.data, src.size, n_src, n_dst,
                                 _raw_stream(device)), "copy_pages")
     return into

@@ -525,3 +525,13 @@ def test_a_page_that_does_not_exist_is_said(K):
         assert not k[1].any()
         with pytest.raises(K.KernelError):
             K.check_device_errors(out.device)
+
+
+def test_as_many_tokens_as_sequences_but_not_one_each_is_said(K):
+    c = Case(1, 2, 64, [10, 20], [2, 0])
+    cache, batch = c.device(K)
+    for call in (lambda: K.split_rotate_store_q8(c.dev["fused"], *cache, batch, 1, 2, 64),
+                 lambda: K.attention_decode_q8(c.dev["fused"], *cache, batch, None, None, 1, 2, 64, 0.1)):
+        call()
+        with pytest.raises(K.KernelError, match="one token for each"):
+            K.check_device_errors("cuda")
