@@ -61,7 +61,7 @@ struct AttnQ8 {
 constexpr int WARPS = 8, MAX_STAGES = 8;
 template <int DP, int NH> struct Q8Shape {
   static constexpr int TILE = DP == 64 ? 32 : 16;        // keys of a warp's step
-  static constexpr int BLOCKS = DP == 256 || NH == 4 ? 1 : 2;   // on an SM
+  static constexpr int BLOCKS = DP == 256 || NH >= 4 ? 1 : 2;   // on an SM
   static constexpr int STAGE_BYTES = 2 * PTB_PAGE * DP;  // a page of one K/V head: keys, then values
   static constexpr int PITCH = DP + 4;                   // floats of a row of the join
 };
@@ -702,7 +702,9 @@ struct Plan {
 Plan plan_of(int dim, int rows) {
   Plan q;
   q.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-  q.nh = rows <= 8 ? 1 : rows <= 16 || q.dp == 256 ? 2 : 4;
+  // heads of 64: fives of eights where they waste less, as for 71 rows: two warps of 40 in place of three of 32, which left two idle
+  const bool fives = q.dp == 64 && ((rows > 32 && rows <= 40) || (rows > 64 && rows <= 80));
+  q.nh = rows <= 8 ? 1 : rows <= 16 || q.dp == 256 ? 2 : fives ? 5 : 4;
   const int groups = (rows + 8 * q.nh - 1) / (8 * q.nh), most = q.dp == 256 ? 8 : 4;
   q.row_groups = groups < most ? groups : most;
   q.rows_pad = q.row_groups * 8 * q.nh;
@@ -710,7 +712,7 @@ Plan plan_of(int dim, int rows) {
   q.page_parts = keys >= parts ? parts : keys >= 2 ? 2 : 1;
   q.rings = keys / q.page_parts;
   // about 96 KB of rings where two blocks are to fit on an SM, else 128
-  const int pages = (q.nh == 4 || q.dp == 256 ? 131072 : 98304) / (2 * PTB_PAGE * q.dp);
+  const int pages = (q.nh >= 4 || q.dp == 256 ? 131072 : 98304) / (2 * PTB_PAGE * q.dp);
   q.stages = pages / q.rings < MAX_STAGES ? pages / q.rings : MAX_STAGES;
   return q;
 }
@@ -783,6 +785,7 @@ int launch_any(const StepBatch& sb, const AttnQ8& p, const Plan& q, dim3 grid, c
   if (q.dp == 64) {
     if (q.nh == 1) PTB_Q8(64, 1);
     if (q.nh == 2) PTB_Q8(64, 2);
+    if (q.nh == 5) PTB_Q8(64, 5);
     PTB_Q8(64, 4);
   }
   if (q.dp == 128) {
@@ -801,7 +804,7 @@ bool known(int heads, int kv_heads, int dim, int pool_pages) {
 // Blocks that share a row's pages: as many as the SMs take at a time, two pages each at least. Up to eight form a cluster and join
 // through its shared memory; more are a multiple of eight, of eight pages each at least, whose clusters join through a workspace.
 int splits_of(long long blocks, int pages, int dp, int nh) {
-  const long long slots = (nh == 4 || dp == 256 ? 1ll : 2ll) * sm_count();
+  const long long slots = (nh >= 4 || dp == 256 ? 1ll : 2ll) * sm_count();
   long long want = blocks > 0 ? slots / blocks : 1;
   if (want > pages / 2) want = pages / 2;
   if (want > MAX_CLUSTER) {
