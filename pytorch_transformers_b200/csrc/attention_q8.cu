@@ -330,7 +330,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   for (int u = 0; u < 2; ++u)
     v_at[u] = ring + PTB_PAGE * DP + (DP == 64 ? place<DP>(kappa<DP>(2 * t4 + u), g4 >> 1) + (g4 & 1) * 8 : place<DP>(kappa<DP>(2 * t4 + u), g4));
   constexpr int EIGHT = 8 * (DP == 64 ? 64 : 128);      // bytes from a row to that of eight keys on
-  const int part_keys = PTB_PAGE / p.page_parts;
+  constexpr bool ONE = DP == 64 || (DP == 128 && NH <= 2);      // a part is one tile: plan_of divides a page as far as it goes
+  const int part_keys = ONE ? TILE : PTB_PAGE / p.page_parts;
   int st = 0, reads_turn = 0;
 
   int i = 0;
@@ -366,7 +367,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
       __syncwarp();
     }
     const int ev = int(int8_t(both & 255)), ek = both >> 8;
-    for (int sub = 0; sub < part_keys; sub += TILE) {
+    for (int sub = 0; sub < (ONE ? TILE : part_keys); sub += TILE) {
     const int key0 = first_key + sub;
     if (key0 > last_pos || key0 + TILE <= low) continue;
     const int kt = st * Shape::STAGE_BYTES + (key0 - page_key0) * (DP == 64 ? 64 : 128);
@@ -399,12 +400,16 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     }
     // The unit of the output: that of the tile's values, but for a difference of 2^3 either way, which the weights carry instead (they
     // stay within float16: 2^8 from the maximum that does not move, 2^3 from here), and for pages 2^60 below the largest.
-    largest = max(largest, ev);
-    const int floor_unit = largest - UNIT_RANGE;
-    const bool new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
-    const int old_unit = unit;
-    if (new_unit) unit = max(ev, floor_unit);
-    const int far = max(ev - unit, -126), shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
+    bool new_unit = false;
+    int far = 0, shift = 0, old_unit = unit;
+    if (ev != unit) {
+      largest = max(largest, ev);
+      const int floor_unit = largest - UNIT_RANGE;
+      new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
+      if (new_unit) unit = max(ev, floor_unit);
+      far = max(ev - unit, -126);
+      shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
+    }
     // score - running maximum + shift, in powers of two; a tile that all rows see whole needs no mask
     const float fk = power_of_two(ek), fshift = float(shift);
     const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
