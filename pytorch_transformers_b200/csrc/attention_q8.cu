@@ -6,26 +6,31 @@
 // Two uses: a step of single tokens (FUSED: rotate the token's queries and key, append key and value to the page, attend, in one
 // launch; a block's rows are the query heads of one K/V head), and prompts or chunks whose queries are given (rows: tokens x heads).
 //
-// What bounds it is the codes' way from memory, so everything is laid out for that. A code becomes a float16 number exactly
-// (cvt.rn.f16x2.e4m3x2), and mma.m16n8k16 takes float16 operands, the codes as its larger one: S^T = K Q^T with 16 keys by 8 rows, and
-// O^T = V^T P^T with 16 entries by 8 rows, since few query heads read a K/V head (with 16 rows by 8 keys, four heads of 128 on each K/V head
-// waste three quarters of the products and twice the registers). The weights' way from one to the other is a transposition of 8 x 8 (movmatrix). Queries are float16 numbers of 11 bits after their row is
-// brought to [1, 2) by a power of two, softmax weights float16 of 11 bits (bfloat16 ones of 8 would cost as much error as the
-// output's own rounding). Sums, maxima and the output are float32.
+// Numbers. A code becomes a float16 number exactly (cvt.rn.f16x2.e4m3x2) and meets float16 operands in mma.m16n8k16: queries of 11
+// bits, their row brought to [1, 2) by a power of two, and softmax weights of 11 bits (of bfloat16's 8 they would cost as much as
+// the output's own rounding). Sums, maxima and the output are float32. Keys' exponents go into the factor of a page's scores; values'
+// are the unit of the float32 output, which is multiplied by a power of two (exactly) where the unit changes. The unit stays within 2^60
+// of the largest exponent seen, so that the output cannot overflow in small units; smaller pages' weights are scaled instead, which no
+// number notices. The running maximum moves only when a score exceeds it by 2^8 (one vote a tile instead of shuffles for each row).
 //
-// Pages land whole, keys and values, in rings that the tensor memory accelerator fills (2 requests a page: with boxes of 16 or
-// 32 rows, asked for by the warp that reads them or by one warp for all, the requests alone took 175 of 200 us where memory allows
-// 150). The warps of a ring take a share of a page's keys each, for one part of the rows or another; they take turns to ask for the next page
-// into the place of one that all have read. So no warp waits for another, but through a ring of pages, before the end. Which key and which entry an index of the
-// matrix instruction stands for is free as long as both operands agree: a thread's share of a key's row is 16 codes in a row (a
-// 16-byte load gives four k-steps of fragments), and its share of a value's row likewise (columns of the output are
-// named accordingly, pairs of keys are put together with byte permutes). Nothing is transposed. The accelerator's swizzle and
-// an order of keys within eight (kappa) keep both ways of reading free of bank conflicts.
+// Products. The codes are the larger operand: S^T = K Q^T of 16 keys by 8 rows, O^T = V^T P^T of 16 entries by 8 rows, since few query
+// heads read a K/V head (as the smaller one, four heads of 128 on each K/V head wasted three quarters of the products and twice the
+// registers). The weights' way from one to the other is a transposition of 8 x 8 (movmatrix). Which key and which entry an index of the
+// instruction stands for is free as long as both operands agree: a thread's share of a key's row is 16 codes in a row (a 16-byte load
+// gives four k-steps of fragments), and its share of a value's row likewise (the output's rows are named accordingly, pairs of keys are
+// put together with byte permutes). The copies' swizzle and an order of keys within eight (kappa) keep both ways of reading free of bank
+// conflicts.
 //
-// Pages have exponents of their own: keys' go into the factor of a page's scores; values' are the unit of the float32
-// output, which is multiplied by a power of two (exactly) where the unit changes. The unit stays within 2^60 of the largest exponent
-// seen, so that the output cannot overflow in small units; smaller pages' weights are scaled instead, which no number notices.
-// The running maximum moves only when a score exceeds it by 2^8 (one vote a tile instead of shuffles for each row).
+// Copies. Pages land whole, keys and values, in rings that the tensor memory accelerator fills, two requests a page; a block's warps
+// have a part of the keys of a ring's pages each, for one group of rows or another, and take turns to ask for the page that comes into
+// the place of one that all have read. No warp waits for another, but through a ring of pages, before the end. Before: cp.async by
+// each warp for itself (a tile's copies a quarter of its time), boxes of 16 or 32 rows asked for by the reading warp or by one warp for
+// all (the requests alone 175 us where memory allows 150).
+//
+// What bounds it: 64 sequences of up to 8,192 keys, 32 heads of 128 on 8, 1 GB of codes: 168 us, 5.8 TB/s; without the arithmetic
+// the same copies take 150, the rate of a plain copy. Half of the ALU's issue slots are taken, by unpacking (80 of 190 instructions for 16
+// keys), maxima, factors and loop. Few rows and short contexts: about 9 us of launch, look-ups one after another (position, page, exponents,
+// codes), queries and the join. 71 heads on one K/V head are bound by mma.sync (3,000 clocks for 32 keys by 40 rows).
 #include <cooperative_groups.h>
 
 #include "q8.cuh"
@@ -148,7 +153,10 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   const int n_rows = min(rows_pad, tokens * qpk - row0);
   if (n_rows <= 0) return;      // all blocks of a cluster alike
   const int past = sb.seq_past[seq], start = sb.seq_start[seq];
-  if (FUSED && sb.seq_new[seq] != 1 && tid == 0) atomicExch(p.error_flag, 24);
+  if (FUSED && sb.seq_new[seq] != 1) {      // as many tokens as sequences, but not one each: `start` may lie past the last row
+    if (tid == 0) atomicExch(p.error_flag, 24);
+    return;
+  }
   const int first_pos = FUSED ? past : past + q0 + row0 / qpk, last_pos = FUSED ? past : past + q0 + (row0 + n_rows - 1) / qpk;
   const int low = p.window > 0 ? max(0, first_pos - p.window + 1) : 0;      // the first key that a row sees
   const int* pages = sb.pages + size_t(seq) * sb.pages_stride;
@@ -279,13 +287,13 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   // Waits are bounded: one that runs out raises the error flag, and the block goes on to its end.
   bool alive = true;
   int turn = 0;      // of the barriers: whether the first pages came twice
-  auto landed = [&](int i, int st, int parity) {
+  auto landed = [&](int st, int parity) {
     const uint32_t bar = bar0 + 8 * st;
     if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 22));
   };
   if (appends) {
     if (new_rose[0] || new_rose[1]) {      // the page's earlier codes have changed: the first pages once more
-      for (int st = 0; st < p.stages && st < n_mine && alive; ++st) landed(st, st, 0);
+      for (int st = 0; st < p.stages && st < n_mine && alive; ++st) landed(st, 0);
       __syncthreads();
       if (leads && alive) ask_first();
       turn = 1;
@@ -343,7 +351,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     if ((i & 31) == 8 && (i & ~31) + 32 < n_mine) look_up((i >> 5) + 1, page_next, exps_next);
     const int both = __shfl_sync(0xffffffffu, exps_now, i & 31);
     const int page_key0 = (pg_begin + ring_no + i * p.rings) * PTB_PAGE;
-    landed(i, st, turn & 1);
+    landed(st, turn & 1);
     if (!alive) break;
     // page `stages` on from the one before, into its place: its warps take turns to ask, a page late, when all have read it
     if (i > 0 && i - 1 + p.stages < n_mine && rg == 0 && ((i - 1) & (p.page_parts - 1)) == part) {      // page_parts is a power of two
@@ -368,186 +376,186 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     }
     const int ev = int(int8_t(both & 255)), ek = both >> 8;
     for (int sub = 0; sub < (ONE ? TILE : part_keys); sub += TILE) {
-    const int key0 = first_key + sub;
-    if (key0 > last_pos || key0 + TILE <= low) continue;
-    const int kt = st * Shape::STAGE_BYTES + (key0 - page_key0) * (DP == 64 ? 64 : 128);
+      const int key0 = first_key + sub;
+      if (key0 > last_pos || key0 + TILE <= low) continue;
+      const int kt = st * Shape::STAGE_BYTES + (key0 - page_key0) * (DP == 64 ? 64 : 128);
 
-    // scores
-    float s[NH][ST][4];      // of row 2 t4, 2 t4 + 1 with key kappa(g4), then with key 8 + kappa(g4)
+      // scores
+      float s[NH][ST][4];      // of row 2 t4, 2 t4 + 1 with key kappa(g4), then with key 8 + kappa(g4)
 #pragma unroll
-    for (int n = 0; n < NH; ++n)
+      for (int n = 0; n < NH; ++n)
 #pragma unroll
-      for (int j = 0; j < ST; ++j) s[n][j][0] = s[n][j][1] = s[n][j][2] = s[n][j][3] = 0.f;
+        for (int j = 0; j < ST; ++j) s[n][j][0] = s[n][j][1] = s[n][j][2] = s[n][j][3] = 0.f;
 #pragma unroll
-    for (int r = 0; r < DP / 64; ++r) {
-      uint4 w[2 * ST];
+      for (int r = 0; r < DP / 64; ++r) {
+        uint4 w[2 * ST];
 #pragma unroll
-      for (int j = 0; j < 2 * ST; ++j) w[j] = *reinterpret_cast<const uint4*>(smem + k_at[r] + kt + j * EIGHT);
+        for (int j = 0; j < 2 * ST; ++j) w[j] = *reinterpret_cast<const uint4*>(smem + k_at[r] + kt + j * EIGHT);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
+        for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+          for (int j = 0; j < ST; ++j) {
+            uint32_t a[4];
+            q8_halves(word_of(w[2 * j], kk), a[0], a[2]);
+            q8_halves(word_of(w[2 * j + 1], kk), a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              const uint4 q = Q_REGS ? qb[Q_REGS ? n : 0][Q_REGS ? r * 2 + kk / 2 : 0] : q_frag(n, r * 4 + kk);
+              mma_f16(s[n][j], a, (kk & 1) ? q.z : q.x, (kk & 1) ? q.w : q.y);
+            }
+          }
+        }
+      }
+      // The unit of the output: that of the tile's values, but for a difference of 2^3 either way, which the weights carry instead (they
+      // stay within float16: 2^8 from the maximum that does not move, 2^3 from here), and for pages 2^60 below the largest.
+      bool new_unit = false;
+      int far = 0, shift = 0, old_unit = unit;
+      if (ev != unit) {
+        largest = max(largest, ev);
+        const int floor_unit = largest - UNIT_RANGE;
+        new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
+        if (new_unit) unit = max(ev, floor_unit);
+        far = max(ev - unit, -126);
+        shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
+      }
+      // score - running maximum + shift, in powers of two; a tile that all rows see whole needs no mask
+      const float fk = power_of_two(ek), fshift = float(shift);
+      const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
+      float over = -INFINITY;      // by how much the tile exceeds the running maxima
+      if (whole && !p.slopes) {
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const bool fresh = m_run[n][h] == -INFINITY;
+            const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < ST; ++j) {
+              s[n][j][h] = fmaf(s[n][j][h], f, m);
+              s[n][j][2 + h] = fmaf(s[n][j][2 + h], f, m);
+              top = fmaxf(top, fmaxf(s[n][j][h], s[n][j][2 + h]));
+            }
+            over = fmaxf(over, fresh ? INFINITY : top);
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = (rg * NH + n) * 8 + 2 * t4 + h;
+            const bool ok = r < n_rows;
+            const int pos = !ok ? -1 : FUSED ? past : past + q0 + (row0 + r) / qpk;
+            const float slope = ok && p.slopes ? p.slopes[g * qpk + (FUSED ? r : (row0 + r) % qpk)] : 0.f;
+            const bool fresh = m_run[n][h] == -INFINITY;
+            const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2 * ST; ++j) {
+              const int key = key0 + j * 8 + kappa<DP>(g4);
+              float v = s[n][j >> 1][(j & 1) * 2 + h] * f;
+              if (p.slopes) v = (v + alibi_bias(slope, key)) * sl2;
+              v += m;
+              if (!whole && (key > pos || (p.window > 0 && key <= pos - p.window))) v = -INFINITY;
+              s[n][j >> 1][(j & 1) * 2 + h] = v;
+              top = fmaxf(top, v);
+            }
+            over = fmaxf(over, fresh && top != -INFINITY ? INFINITY : top);
+          }
+      }
+      if (__any_sync(0xffffffffu, over > MOVE_LOG2 + fshift) || new_unit) {
+        const float change = power_of_two(min(max(old_unit - unit, -126), 126));
+#pragma unroll
+        for (int n = 0; n < NH; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float up = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < ST; ++j) up = fmaxf(up, fmaxf(s[n][j][h], s[n][j][2 + h]));
+#pragma unroll
+            for (int lanes = 4; lanes < 32; lanes *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, lanes));
+            up -= fshift;
+            const bool fresh = m_run[n][h] == -INFINITY;      // then `up` is the maximum itself
+            if (!fresh) up = fmaxf(up, 0.f);
+            const float corr = fresh ? 0.f : exp2f(-up), by = up == -INFINITY ? 0.f : up;
+            m_run[n][h] = fresh ? up : m_run[n][h] + up;
+            l_run[n][h] *= corr;
+#pragma unroll
+            for (int j = 0; j < ST; ++j) {
+              s[n][j][h] -= by;
+              s[n][j][2 + h] -= by;
+            }
+            const float f = corr * change;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              o[n][j][h] *= f;
+              o[n][j][2 + h] *= f;
+            }
+          }
+      }
+      uint32_t pb[NH][ST][2];
+      const float back = power_of_two(-shift);      // the sums are of the weights themselves
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
 #pragma unroll
         for (int j = 0; j < ST; ++j) {
-          uint32_t a[4];
-          q8_halves(word_of(w[2 * j], kk), a[0], a[2]);
-          q8_halves(word_of(w[2 * j + 1], kk), a[1], a[3]);
 #pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            const uint4 q = Q_REGS ? qb[Q_REGS ? n : 0][Q_REGS ? r * 2 + kk / 2 : 0] : q_frag(n, r * 4 + kk);
-            mma_f16(s[n][j], a, (kk & 1) ? q.z : q.x, (kk & 1) ? q.w : q.y);
-          }
+          for (int e = 0; e < 4; ++e) s[n][j][e] = fast_exp2(s[n][j][e]);
+          l_run[n][0] = fmaf(s[n][j][0] + s[n][j][2], back, l_run[n][0]);
+          l_run[n][1] = fmaf(s[n][j][1] + s[n][j][3], back, l_run[n][1]);
+        }
+        if (far != shift) {      // a page 2^60 below the largest: its weights are scaled before they are rounded
+#pragma unroll
+          for (int j = 0; j < ST; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][j][e] *= power_of_two(far);
+        }
+#pragma unroll
+        for (int j = 0; j < ST; ++j) {
+          pb[n][j][0] = transposed(pack_half(s[n][j][0], s[n][j][1]));
+          pb[n][j][1] = transposed(pack_half(s[n][j][2], s[n][j][3]));
         }
       }
-    }
-    // The unit of the output: that of the tile's values, but for a difference of 2^3 either way, which the weights carry instead (they
-    // stay within float16: 2^8 from the maximum that does not move, 2^3 from here), and for pages 2^60 below the largest.
-    bool new_unit = false;
-    int far = 0, shift = 0, old_unit = unit;
-    if (ev != unit) {
-      largest = max(largest, ev);
-      const int floor_unit = largest - UNIT_RANGE;
-      new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
-      if (new_unit) unit = max(ev, floor_unit);
-      far = max(ev - unit, -126);
-      shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
-    }
-    // score - running maximum + shift, in powers of two; a tile that all rows see whole needs no mask
-    const float fk = power_of_two(ek), fshift = float(shift);
-    const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
-    float over = -INFINITY;      // by how much the tile exceeds the running maxima
-    if (whole && !p.slopes) {
+      // output. Keys that no row of the block sees are taken as zero: their codes may be anything.
+      const bool edge = key0 + TILE - 1 > last_pos || key0 < low;
 #pragma unroll
-      for (int n = 0; n < NH; ++n)
+      for (int ks = 0; ks < ST; ++ks)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const bool fresh = m_run[n][h] == -INFINITY;
-          const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < ST; ++j) {
-            s[n][j][h] = fmaf(s[n][j][h], f, m);
-            s[n][j][2 + h] = fmaf(s[n][j][2 + h], f, m);
-            top = fmaxf(top, fmaxf(s[n][j][h], s[n][j][2 + h]));
-          }
-          over = fmaxf(over, fresh ? INFINITY : top);
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NH; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = (rg * NH + n) * 8 + 2 * t4 + h;
-          const bool ok = r < n_rows;
-          const int pos = !ok ? -1 : FUSED ? past : past + q0 + (row0 + r) / qpk;
-          const float slope = ok && p.slopes ? p.slopes[g * qpk + (FUSED ? r : (row0 + r) % qpk)] : 0.f;
-          const bool fresh = m_run[n][h] == -INFINITY;
-          const float f = row_fac[n][h] * fk, m = fresh ? fshift : fshift - m_run[n][h];
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 2 * ST; ++j) {
-            const int key = key0 + j * 8 + kappa<DP>(g4);
-            float v = s[n][j >> 1][(j & 1) * 2 + h] * f;
-            if (p.slopes) v = (v + alibi_bias(slope, key)) * sl2;
-            v += m;
-            if (!whole && (key > pos || (p.window > 0 && key <= pos - p.window))) v = -INFINITY;
-            s[n][j >> 1][(j & 1) * 2 + h] = v;
-            top = fmaxf(top, v);
-          }
-          over = fmaxf(over, fresh && top != -INFINITY ? INFINITY : top);
-        }
-    }
-    if (__any_sync(0xffffffffu, over > MOVE_LOG2 + fshift) || new_unit) {
-      const float change = power_of_two(min(max(old_unit - unit, -126), 126));
-#pragma unroll
-      for (int n = 0; n < NH; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float up = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < ST; ++j) up = fmaxf(up, fmaxf(s[n][j][h], s[n][j][2 + h]));
-#pragma unroll
-          for (int lanes = 4; lanes < 32; lanes *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, lanes));
-          up -= fshift;
-          const bool fresh = m_run[n][h] == -INFINITY;      // then `up` is the maximum itself
-          if (!fresh) up = fmaxf(up, 0.f);
-          const float corr = fresh ? 0.f : exp2f(-up), by = up == -INFINITY ? 0.f : up;
-          m_run[n][h] = fresh ? up : m_run[n][h] + up;
-          l_run[n][h] *= corr;
-#pragma unroll
-          for (int j = 0; j < ST; ++j) {
-            s[n][j][h] -= by;
-            s[n][j][2 + h] -= by;
-          }
-          const float f = corr * change;
-#pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            o[n][j][h] *= f;
-            o[n][j][2 + h] *= f;
-          }
-        }
-    }
-    uint32_t pb[NH][ST][2];
-    const float back = power_of_two(-shift);      // the sums are of the weights themselves
-#pragma unroll
-    for (int n = 0; n < NH; ++n) {
-#pragma unroll
-      for (int j = 0; j < ST; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][j][e] = fast_exp2(s[n][j][e]);
-        l_run[n][0] = fmaf(s[n][j][0] + s[n][j][2], back, l_run[n][0]);
-        l_run[n][1] = fmaf(s[n][j][1] + s[n][j][3], back, l_run[n][1]);
-      }
-      if (far != shift) {      // a page 2^60 below the largest: its weights are scaled before they are rounded
-#pragma unroll
-        for (int j = 0; j < ST; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][j][e] *= power_of_two(far);
-      }
-#pragma unroll
-      for (int j = 0; j < ST; ++j) {
-        pb[n][j][0] = transposed(pack_half(s[n][j][0], s[n][j][1]));
-        pb[n][j][1] = transposed(pack_half(s[n][j][2], s[n][j][3]));
-      }
-    }
-    // output. Keys that no row of the block sees are taken as zero: their codes may be anything.
-    const bool edge = key0 + TILE - 1 > last_pos || key0 < low;
-#pragma unroll
-    for (int ks = 0; ks < ST; ++ks)
-#pragma unroll
-      for (int rr = 0; rr < VR; ++rr) {
-        uint32_t v[4][VW];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int at = v_at[u & 1] + kt + rr * (PTB_PAGE * 128) + (2 * ks + (u >> 1)) * EIGHT;
-          if (DP == 64) {
-            const uint2 x = *reinterpret_cast<const uint2*>(smem + at);
-            v[u][0] = x.x; v[u][1] = x.y;
-          } else {
-            const uint4 x = *reinterpret_cast<const uint4*>(smem + at);
-            v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
-          }
-        }
-        if (edge) {
+        for (int rr = 0; rr < VR; ++rr) {
+          uint32_t v[4][VW];
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int key = key0 + (2 * ks + (u >> 1)) * 8 + kappa<DP>(2 * t4 + (u & 1));
+            const int at = v_at[u & 1] + kt + rr * (PTB_PAGE * 128) + (2 * ks + (u >> 1)) * EIGHT;
+            if (DP == 64) {
+              const uint2 x = *reinterpret_cast<const uint2*>(smem + at);
+              v[u][0] = x.x; v[u][1] = x.y;
+            } else {
+              const uint4 x = *reinterpret_cast<const uint4*>(smem + at);
+              v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
+            }
+          }
+          if (edge) {
 #pragma unroll
-            for (int q = 0; q < VW; ++q) v[u][q] = key > last_pos || key < low ? 0u : v[u][q];
+            for (int u = 0; u < 4; ++u) {
+              const int key = key0 + (2 * ks + (u >> 1)) * 8 + kappa<DP>(2 * t4 + (u & 1));
+#pragma unroll
+              for (int q = 0; q < VW; ++q) v[u][q] = key > last_pos || key < low ? 0u : v[u][q];
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < VW; ++q) {
+            uint32_t a[4], b[4];      // entries 4 q, 4 q + 1 and 4 q + 2, 4 q + 3 of the thread's
+            q8_halves(__byte_perm(v[0][q], v[1][q], 0x5140), a[0], a[1]);
+            q8_halves(__byte_perm(v[2][q], v[3][q], 0x5140), a[2], a[3]);
+            q8_halves(__byte_perm(v[0][q], v[1][q], 0x7362), b[0], b[1]);
+            q8_halves(__byte_perm(v[2][q], v[3][q], 0x7362), b[2], b[3]);
+#pragma unroll
+            for (int n = 0; n < NH; ++n) {
+              mma_f16(o[n][rr * 8 + q * 2], a, pb[n][ks][0], pb[n][ks][1]);
+              mma_f16(o[n][rr * 8 + q * 2 + 1], b, pb[n][ks][0], pb[n][ks][1]);
+            }
           }
         }
-#pragma unroll
-        for (int q = 0; q < VW; ++q) {
-          uint32_t a[4], b[4];      // entries 4 q, 4 q + 1 and 4 q + 2, 4 q + 3 of the thread's
-          q8_halves(__byte_perm(v[0][q], v[1][q], 0x5140), a[0], a[1]);
-          q8_halves(__byte_perm(v[2][q], v[3][q], 0x5140), a[2], a[3]);
-          q8_halves(__byte_perm(v[0][q], v[1][q], 0x7362), b[0], b[1]);
-          q8_halves(__byte_perm(v[2][q], v[3][q], 0x7362), b[2], b[3]);
-#pragma unroll
-          for (int n = 0; n < NH; ++n) {
-            mma_f16(o[n][rr * 8 + q * 2], a, pb[n][ks][0], pb[n][ks][1]);
-            mma_f16(o[n][rr * 8 + q * 2 + 1], b, pb[n][ks][0], pb[n][ks][1]);
-          }
-        }
-      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(bar0 + 8 * (MAX_STAGES + st));
@@ -555,7 +563,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   }
   if (!alive)      // a wait ran out: what is in flight lands before the block ends (bounded waits again)
     for (int k = 0; k < p.stages && i + k < n_mine; ++k) {
-      landed(i + k, st, turn & 1);
+      landed(st, turn & 1);
       if (++st == p.stages) st = 0, ++turn;
     }
 

@@ -214,9 +214,12 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
   } else {
     int local = job;
     auto low = [&](int s) { return p.window > 0 ? max(0, sb.seq_past[s] - p.window + 1) / PTB_PAGE : 0; };
-    const int seq = find_job(sb.n_seqs, local, [&](int s) {
-      return sb.seq_new[s] > 0 ? (sb.seq_past[s] + sb.seq_new[s] + PTB_PAGE - 1) / PTB_PAGE - low(s) : 0;
-    });
+    auto count = [&](int s) { return sb.seq_new[s] > 0 ? (sb.seq_past[s] + sb.seq_new[s] + PTB_PAGE - 1) / PTB_PAGE - low(s) : 0; };
+    if (g == 0 && job + 1 == int(gridDim.x)) {      // 25: the step spans more pages than the workspace has
+      int more = job + 1;
+      if (find_job(sb.n_seqs, more, count) >= 0 && tid == 0) atomicExch(p.error_flag, 25);
+    }
+    const int seq = find_job(sb.n_seqs, local, count);
     if (seq < 0) return;
     const int index = low(seq) + local;
     page = sb.pages[size_t(seq) * sb.pages_stride + index];

@@ -535,6 +535,8 @@ def check_device_errors(device) -> None:
             flag.zero_()
             if code == 21:
                 raise KernelError("a page table or list named a page that the cache does not have: the results are void")
+            if code == 25:
+                raise KernelError("attention_q8: the step's sequences span more pages than n_pages: the results are void")
             if code == 24:
                 raise KernelError("a step of as many tokens as sequences did not bring one token for each: its results are void")
             raise KernelError(f"a kernel gave up waiting inside its pipeline (code {code}): its results are void")
@@ -1984,8 +1986,8 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     if not (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 3 and q.is_contiguous() and q.shape[0] == batch.n_tokens):
         raise KernelError(f"{what} takes contiguous bfloat16 queries [tokens, heads, head_dim] of the step's tokens")
     n, heads, head_dim = q.shape
-    if heads % kv_heads or window < 0:
-        raise KernelError(f"{what}: {heads} heads on {kv_heads} K/V heads, window {window}")
+    if heads % kv_heads or window < 0 or n_splits < 0:
+        raise KernelError(f"{what}: {heads} heads on {kv_heads} K/V heads, window {window}, {n_splits} splits")
     device = q.get_device()
     pool_pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     slopes_at = _check_slopes(slopes, heads, device, what)

@@ -535,3 +535,17 @@ def test_as_many_tokens_as_sequences_but_not_one_each_is_said(K):
         call()
         with pytest.raises(K.KernelError, match="one token for each"):
             K.check_device_errors("cuda")
+
+
+def test_fewer_pages_than_a_step_spans_are_said(K):
+    for short, said in ((0, False), (1, True)):
+        c = Case(1, 2, 64, [100, 0], [130, 200])
+        cache, batch = c.device(K)
+        q = torch.zeros(330, 2, 64, dtype=BF).cuda()
+        lists = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([0, 0, 1, 1], [0, 128, 0, 128])]
+        K.attention_q8(q, *cache, batch, *lists, 4, 128, None, 1, 0.1, n_pages=4 + 4 - short)
+        if said:
+            with pytest.raises(K.KernelError, match="more pages than n_pages"):
+                K.check_device_errors("cuda")
+        else:
+            K.check_device_errors("cuda")
