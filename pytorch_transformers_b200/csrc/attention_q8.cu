@@ -156,7 +156,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   if (n_rows <= 0) return;      // all blocks of a cluster alike
   const int past = sb.seq_past[seq], start = sb.seq_start[seq];
   if (FUSED && sb.seq_new[seq] != 1) {      // as many tokens as sequences, but not one each: `start` may lie past the last row
-    if (tid == 0) atomicExch(p.error_flag, 24);
+    if (tid == 0) atomicExch(p.error_flag, 54);
     return;
   }
   const int first_pos = FUSED ? past : past + q0 + row0 / qpk, last_pos = FUSED ? past : past + q0 + (row0 + n_rows - 1) / qpk;
@@ -182,7 +182,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     if (i < n_mine) {
       page = pages[pg_begin + ring_no + i * p.rings];
       if (page < 0 || page >= p.pool_pages) {
-        atomicExch(p.error_flag, 21);
+        atomicExch(p.error_flag, 51);
         page = 0;
       }
       const size_t block = size_t(page) * p.kv_heads + g;
@@ -291,7 +291,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   int turn = 0;      // of the barriers: whether the first pages came twice
   auto landed = [&](int st, int parity) {
     const uint32_t bar = bar0 + 8 * st;
-    if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 22));
+    if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 52));
   };
   if (appends) {
     if (new_rose[0] || new_rose[1]) {      // the page's earlier codes have changed: the first pages once more
@@ -360,7 +360,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
       const int j = i - 1 + p.stages, before = st == 0 ? p.stages - 1 : st - 1;
       const int page = __shfl_sync(0xffffffffu, (j ^ i) < 32 ? page_now : page_next, j & 31);
       const uint32_t bar = bar0 + 8 * (MAX_STAGES + before), parity = (st == 0 ? reads_turn - 1 : reads_turn) & 1;
-      if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 23));
+      if (!__all_sync(0xffffffffu, mbar_test(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.error_flag, 53));
       if (!alive) break;
       if (lane == 0) ask(page, before);
     }

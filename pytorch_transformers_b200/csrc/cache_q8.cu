@@ -81,8 +81,8 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
     if (seq >= sb.n_seqs) return;
     const bool keys = (at & 1) == 0;
     const int past = sb.seq_past[seq], page = sb.pages[size_t(seq) * sb.pages_stride + past / PTB_PAGE];
-    if (page < 0 || page >= p.pool_pages || sb.seq_new[seq] != 1) {      // 24: as many tokens as sequences, but not one each
-      if ((tid & 31) == 0) atomicExch(p.error_flag, sb.seq_new[seq] != 1 ? 24 : 21);
+    if (page < 0 || page >= p.pool_pages || sb.seq_new[seq] != 1) {      // 54: as many tokens as sequences, but not one each
+      if ((tid & 31) == 0) atomicExch(p.error_flag, sb.seq_new[seq] != 1 ? 54 : 51);
       return;
     }
     const size_t block = size_t(page) * p.kv_heads + g, t = sb.seq_start[seq];
@@ -105,7 +105,7 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
   const int index = past / PTB_PAGE + local;
   const int page = sb.pages[size_t(seq) * sb.pages_stride + index];
   if (page < 0 || page >= p.pool_pages) {      // a table that names no page: said, and nothing is written
-    if (tid == 0) atomicExch(p.error_flag, 21);
+    if (tid == 0) atomicExch(p.error_flag, 51);
     return;
   }
   const int first = max(past - index * PTB_PAGE, 0), last = min(past + n_new - index * PTB_PAGE, PTB_PAGE);   // the new rows of the page
@@ -215,9 +215,9 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
     int local = job;
     auto low = [&](int s) { return p.window > 0 ? max(0, sb.seq_past[s] - p.window + 1) / PTB_PAGE : 0; };
     auto count = [&](int s) { return sb.seq_new[s] > 0 ? (sb.seq_past[s] + sb.seq_new[s] + PTB_PAGE - 1) / PTB_PAGE - low(s) : 0; };
-    if (g == 0 && job + 1 == int(gridDim.x)) {      // 25: the step spans more pages than the workspace has
+    if (g == 0 && job + 1 == int(gridDim.x)) {      // 55: the step spans more pages than the workspace has
       int more = job + 1;
-      if (find_job(sb.n_seqs, more, count) >= 0 && tid == 0) atomicExch(p.error_flag, 25);
+      if (find_job(sb.n_seqs, more, count) >= 0 && tid == 0) atomicExch(p.error_flag, 55);
     }
     const int seq = find_job(sb.n_seqs, local, count);
     if (seq < 0) return;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
   }
   const bool known = page >= 0 && page < p.pool_pages;
   if (!known) {
-    if (g == 0 && tid == 0) atomicExch(p.error_flag, 21);
+    if (g == 0 && tid == 0) atomicExch(p.error_flag, 51);
     valid = 0;
     page = 0;
   }

@@ -533,11 +533,11 @@ def check_device_errors(device) -> None:
         code = int(flag.item())
         if code != 0:
             flag.zero_()
-            if code == 21:
+            if code == 51:
                 raise KernelError("a page table or list named a page that the cache does not have: the results are void")
-            if code == 25:
+            if code == 55:
                 raise KernelError("attention_q8: the step's sequences span more pages than n_pages: the results are void")
-            if code == 24:
+            if code == 54:
                 raise KernelError("a step of as many tokens as sequences did not bring one token for each: its results are void")
             raise KernelError(f"a kernel gave up waiting inside its pipeline (code {code}): its results are void")
 

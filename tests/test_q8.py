@@ -42,3 +42,21 @@ def test_rounding_agrees_with_torch():
     x = x.clamp(-464, 464)
     assert torch.equal(plain.round_e4m3(x).float(), x.to(K.Q8).float())
     assert math.isnan(float(plain.round_e4m3(torch.tensor([math.inf]))[0]))
+
+
+def test_error_codes_are_nobody_elses():
+    # a wait that runs out in another kernel must not read as a page number that is none
+    import pathlib
+    import re
+    used = {}
+    for path in (pathlib.Path(K.__file__).parent / "csrc").glob("*.cu*"):
+        for code in re.findall(r"error_flag, (\d+)\)", path.read_text()):
+            used.setdefault(int(code), set()).add(path.name)
+    own = {"attention_q8.cu", "cache_q8.cu"}
+    assert {51, 52, 53, 54, 55} <= set(used) and all(used[c] <= own for c in used if used[c] & own)
+
+
+def test_a_wait_that_ran_out_elsewhere_is_not_called_a_page(monkeypatch):
+    monkeypatch.setattr(K, "_error_flags", {torch.device("cpu"): torch.tensor([21], dtype=torch.int32)})
+    with pytest.raises(K.KernelError, match="gave up waiting"):
+        K.check_device_errors("cpu")
