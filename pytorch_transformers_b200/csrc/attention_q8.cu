@@ -180,7 +180,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     page = 0;
     exps = 0;
     if (i < n_mine) {
-      page = pages[pg_begin + ring_no + i * p.rings];
+      const int at = pg_begin + ring_no + i * p.rings;
+      page = at < sb.pages_stride ? pages[at] : -1;
       if (page < 0 || page >= p.pool_pages) {
         atomicExch(p.error_flag, 51);
         page = 0;
@@ -214,7 +215,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
     ask_first();
   }
   if (appends) {
-    const int page = pages[pg_end - 1];
+    const int page = pg_end <= sb.pages_stride ? pages[pg_end - 1] : -1;
     const __nv_bfloat16* frow = p.rows + size_t(start) * fused_width + size_t(g) * (qpk + 2) * D;
     if (warp == 5 || warp == 7) {      // never the ones that ask for the first pages
       const int which = warp == 7;

@@ -80,7 +80,8 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
     const int at = blockIdx.x * (STORE_THREADS / 32) + tid / 32, seq = at / (2 * p.kv_heads), g = at % (2 * p.kv_heads) >> 1;
     if (seq >= sb.n_seqs) return;
     const bool keys = (at & 1) == 0;
-    const int past = sb.seq_past[seq], page = sb.pages[size_t(seq) * sb.pages_stride + past / PTB_PAGE];
+    const int past = sb.seq_past[seq], index = past / PTB_PAGE;
+    const int page = index < sb.pages_stride ? sb.pages[size_t(seq) * sb.pages_stride + index] : -1;
     if (page < 0 || page >= p.pool_pages || sb.seq_new[seq] != 1) {      // 54: as many tokens as sequences, but not one each
       if ((tid & 31) == 0) atomicExch(p.error_flag, sb.seq_new[seq] != 1 ? 54 : 51);
       return;
@@ -103,7 +104,7 @@ template <int MOST> __global__ void __launch_bounds__(STORE_THREADS) store_q8_ke
   if (seq < 0) return;
   const int past = sb.seq_past[seq], n_new = sb.seq_new[seq], start = sb.seq_start[seq];
   const int index = past / PTB_PAGE + local;
-  const int page = sb.pages[size_t(seq) * sb.pages_stride + index];
+  const int page = index < sb.pages_stride ? sb.pages[size_t(seq) * sb.pages_stride + index] : -1;
   if (page < 0 || page >= p.pool_pages) {      // a table that names no page: said, and nothing is written
     if (tid == 0) atomicExch(p.error_flag, 51);
     return;
@@ -222,9 +223,10 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
     const int seq = find_job(sb.n_seqs, local, count);
     if (seq < 0) return;
     const int index = low(seq) + local;
-    page = sb.pages[size_t(seq) * sb.pages_stride + index];
+    const bool listed = index < sb.pages_stride;      // a table too narrow for its sequence is neither read nor written past a row's end
+    page = listed ? sb.pages[size_t(seq) * sb.pages_stride + index] : -1;
     valid = min(PTB_PAGE, sb.seq_past[seq] + sb.seq_new[seq] - index * PTB_PAGE);
-    if (g == 0 && tid == 0) p.table[size_t(seq) * sb.pages_stride + index] = job;
+    if (listed && g == 0 && tid == 0) p.table[size_t(seq) * sb.pages_stride + index] = job;
   }
   const bool known = page >= 0 && page < p.pool_pages;
   if (!known) {

@@ -1845,7 +1845,7 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
                pages: torch.Tensor) -> StepBatchC:
     """The description of a step for the kernels from int32 tensors on the device (``StepContext`` builds it for the engine):
     sequence and position of every token, each sequence's first token, tokens of this step and tokens before it, and the page
-    table [sequences, width]. The tensors must outlive the kernels that read them."""
+    table [sequences, width], wide enough for every sequence's tokens. The tensors must outlive the kernels that read them."""
     for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages):
         if not (t.dtype is torch.int32 and t.is_cuda and t.is_contiguous()):
             raise KernelError("step_batch takes contiguous int32 tensors on the device")

@@ -549,3 +549,19 @@ def test_fewer_pages_than_a_step_spans_are_said(K):
                 K.check_device_errors("cuda")
         else:
             K.check_device_errors("cuda")
+
+
+def test_a_table_too_narrow_for_its_sequence_is_said(K):
+    # two sequences of two and three pages behind a table one page wide: nothing past its rows is read, and only page 0, which the
+    # missing ones read as, may be part of the result; the cache stays as it was
+    c = Case(1, 2, 64, [100, 140], [1, 1])
+    c.table = c.table[:, :1].contiguous()
+    cache, batch = c.device(K)
+    before = [t.clone() for t in cache]
+    for call in (lambda: K.split_rotate_store_q8(c.dev["fused"], *cache, batch, 1, 2, 64),
+                 lambda: K.attention_decode_q8(c.dev["fused"], *cache, batch, None, None, 1, 2, 64, 0.1)):
+        call()
+        with pytest.raises(K.KernelError, match="page"):
+            K.check_device_errors("cuda")
+        for a, b in zip(cache, before):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
