@@ -1849,11 +1849,16 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
     for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages):
         if not (t.dtype is torch.int32 and t.is_cuda and t.is_contiguous()):
             raise KernelError("step_batch takes contiguous int32 tensors on the device")
+    device = pages.get_device()
+    if any(t.get_device() != device for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past)):
+        raise KernelError("step_batch takes tensors of one device")
     n, tokens, table = seq_start.numel(), tok_seq.numel(), pages.shape
     if tok_pos.numel() != tokens or seq_new.numel() != n or seq_past.numel() != n or len(table) != 2 or table[0] != n:
         raise KernelError("step_batch: the arrays' lengths do not fit one another")
-    return StepBatchC(tok_seq.data_ptr(), tok_pos.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), seq_past.data_ptr(),
-                      pages.data_ptr(), table[1], tokens, n)
+    batch = StepBatchC(tok_seq.data_ptr(), tok_pos.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), seq_past.data_ptr(),
+                       pages.data_ptr(), table[1], tokens, n)
+    batch.device = device
+    return batch
 
 
 def _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads: int, head_dim: int, device: int, what: str) -> int:
@@ -1890,6 +1895,12 @@ def _check_fused_q8(fused, batch, rope, kv_heads: int, q_per_kv: int, head_dim: 
     return cos.data_ptr(), sin.data_ptr(), shape[1]
 
 
+def _check_batch(batch, device: int, what: str) -> None:
+    """A step that ``step_batch`` described lies on the device of the call's tensors."""
+    if getattr(batch, "device", device) != device:
+        raise KernelError(f"{what}: the step was described on device {batch.device}, the other tensors are on {device}")
+
+
 def _check_slopes(slopes, heads: int, device: int, what: str):
     if slopes is None:
         return None
@@ -1910,6 +1921,7 @@ def split_rotate_store_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torc
     what = "split_rotate_store_q8"
     cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
     device = fused.get_device()
+    _check_batch(batch, device, what)
     pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     q = fused.new_empty((fused.shape[0], kv_heads * q_per_kv, head_dim))
     cache = (k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr()) if write_cache else (None,) * 4
@@ -1947,6 +1959,7 @@ def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.
     what = "attention_decode_q8"
     cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
     device = fused.get_device()
+    _check_batch(batch, device, what)
     pool_pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     heads = kv_heads * q_per_kv
     slopes_at = _check_slopes(slopes, heads, device, what)
@@ -1981,7 +1994,8 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     head_dim] bfloat16; tiles of ``tile_tokens`` consecutive new tokens as for the other prompt kernels. ``n_pages``: the pages that the
     step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of up to 128 take their
     pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. ``n_splits``: as ``attention_decode_q8``
-    takes it, for the others. Returns [tokens, heads * head_dim]."""
+    takes it, for the others. A value held as no number reaches the rows of a tile that share its matrix instructions, whether they see
+    it or not (single tokens: the rows that see it). Returns [tokens, heads * head_dim]."""
     what = "attention_q8"
     if not (q.is_cuda and q.dtype is torch.bfloat16 and q.dim() == 3 and q.is_contiguous() and q.shape[0] == batch.n_tokens):
         raise KernelError(f"{what} takes contiguous bfloat16 queries [tokens, heads, head_dim] of the step's tokens")
@@ -1989,6 +2003,7 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     if heads % kv_heads or window < 0 or n_splits < 0:
         raise KernelError(f"{what}: {heads} heads on {kv_heads} K/V heads, window {window}, {n_splits} splits")
     device = q.get_device()
+    _check_batch(batch, device, what)
     pool_pages = _check_q8(k_pool, k_exp, v_pool, v_exp, kv_heads, head_dim, device, what)
     slopes_at = _check_slopes(slopes, heads, device, what)
     for t in (tile_seq, tile_q0):

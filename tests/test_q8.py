@@ -60,3 +60,37 @@ def test_a_wait_that_ran_out_elsewhere_is_not_called_a_page(monkeypatch):
     monkeypatch.setattr(K, "_error_flags", {torch.device("cpu"): torch.tensor([21], dtype=torch.int32)})
     with pytest.raises(K.KernelError, match="gave up waiting"):
         K.check_device_errors("cpu")
+
+
+class _Ints:
+    """As much of an int32 tensor on a CUDA device as the descriptions of steps look at."""
+    dtype, is_cuda = torch.int32, True
+
+    def __init__(self, device, *shape):
+        self.device_number, self.shape = device, shape
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.device_number
+
+    def numel(self):
+        return math.prod(self.shape)
+
+    def data_ptr(self):
+        return 256
+
+
+def test_steps_described_on_two_devices_are_refused():
+    arrays = [_Ints(0, 3), _Ints(0, 3), _Ints(0, 2), _Ints(0, 2), _Ints(0, 2), _Ints(0, 2, 4)]
+    batch = K.step_batch(*arrays)
+    assert (batch.n_tokens, batch.n_seqs, batch.pages_stride) == (3, 2, 4)
+    K._check_batch(batch, 0, "here")
+    with pytest.raises(K.KernelError, match="device"):
+        K._check_batch(batch, 1, "there")
+    for i in range(6):
+        other = list(arrays)
+        other[i] = _Ints(1, *arrays[i].shape)
+        with pytest.raises(K.KernelError, match="one device"):
+            K.step_batch(*other)
