@@ -290,13 +290,13 @@ class Cache:
         self.epoch += 1
 
     def _renumber(self, num_pages: int) -> int:
+        self.epoch += 1      # first: a group may run out of memory after another has moved
         count = 0
         for gi, g in enumerate(self.groups):
             moved = g.renumber(num_pages)
             count += len(moved)
             for rec in self.records.values():
                 rec.pages[gi] = [moved.get(p, p) for p in rec.pages[gi]]
-        self.epoch += 1
         return count
 
     def compact(self) -> int:

@@ -161,3 +161,31 @@ def test_which_caches_hold_8_bits():
     assert resolve_cache_dtype("float8_e4m3fn", torch.bfloat16) == f8
     with pytest.raises(ValueError):
         resolve_cache_dtype("int4", torch.bfloat16)
+
+
+def test_a_resize_without_memory_for_the_second_group_leaves_what_is_held(monkeypatch):
+    needs = [(0, CacheNeed("full", 1, 8), None), (1, CacheNeed("window", 1, 8, 100), None)]
+    cache = Cache(needs, 6 * PAGE, torch.float32, "cpu")
+    other = cache.open()
+    slot = cache.open()
+    for s in (other, slot):
+        cache.reserve(s, 130)
+        cache.commit(s, 130)
+    for g in cache.groups:
+        for i, p in enumerate(cache.pages(slot, cache.groups.index(g))):
+            if p >= 0:
+                g.k[:, p] = i + 1
+    cache.close(other)                   # the lowest pages are free: those that are held will move
+    epoch = cache.epoch
+    with monkeypatch.context() as m:
+        m.setattr(cache.groups[1], "_storage", lambda n: (_ for _ in ()).throw(MemoryError("none")))
+        with pytest.raises(MemoryError):
+            cache.resize(20 * PAGE)
+    assert cache.epoch > epoch           # the first group's pages have moved: what was prepared for the old ones is stale
+    cache.check()
+    cache.resize(20 * PAGE)
+    cache.check()
+    for gi, g in enumerate(cache.groups):
+        assert g.pool.capacity == 20
+        for i, p in enumerate(cache.pages(slot, gi)):
+            assert p < 0 or bool((g.k[:, p] == i + 1).all())
