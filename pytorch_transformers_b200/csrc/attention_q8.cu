@@ -71,6 +71,7 @@ template <int DP, int NH> struct Q8Shape {
   static constexpr int BLOCKS = DP == 256 || NH >= 4 ? 1 : 2;   // on an SM
   static constexpr int STAGE_BYTES = 2 * PTB_PAGE * DP;  // a page of one K/V head: keys, then values
   static constexpr int PITCH = DP + 4;                   // floats of a row of the join
+  static constexpr bool ONE = DP == 64 || (DP == 128 && NH <= 2);      // a warp's part of a page is one tile; the launch checks it
 };
 
 // The order of a tile's keys: column c of eight stands for key kappa(c). A quarter-warp's 16-byte reads of keys touch columns 2 t and
@@ -341,7 +342,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
   for (int u = 0; u < 2; ++u)
     v_at[u] = ring + PTB_PAGE * DP + (DP == 64 ? place<DP>(kappa<DP>(2 * t4 + u), g4 >> 1) + (g4 & 1) * 8 : place<DP>(kappa<DP>(2 * t4 + u), g4));
   constexpr int EIGHT = 8 * (DP == 64 ? 64 : 128);      // bytes from a row to that of eight keys on
-  constexpr bool ONE = DP == 64 || (DP == 128 && NH <= 2);      // a part is one tile: plan_of divides a page as far as it goes
+  constexpr bool ONE = Shape::ONE;
   const int part_keys = ONE ? TILE : PTB_PAGE / p.page_parts;
   int st = 0, reads_turn = 0;
 
@@ -758,6 +759,7 @@ template <int DP, int NH, bool FUSED>
 int launch_attn(const StepBatch& sb, AttnQ8 p, const Plan& q, dim3 grid, cudaStream_t stream) {
   using Shape = Q8Shape<DP, NH>;
   const int key_groups = q.page_parts * q.rings;
+  if (Shape::ONE && PTB_PAGE / q.page_parts != Shape::TILE) return PTB_ERR_SIZE;      // keys would be left out
   const size_t ring = size_t(q.rings) * q.stages * Shape::STAGE_BYTES;
   const size_t join = size_t(key_groups) * q.rows_pad * Shape::PITCH * sizeof(float);
   p.ring_bytes = int(ring > join ? ring : (join + 15) / 16 * 16);
