@@ -1850,7 +1850,7 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
         if not (t.dtype is torch.int32 and t.is_cuda and t.is_contiguous()):
             raise KernelError("step_batch takes contiguous int32 tensors on the device")
     device = pages.get_device()
-    if any(t.get_device() != device for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past)):
+    if not (tok_seq.get_device() == tok_pos.get_device() == seq_start.get_device() == seq_new.get_device() == seq_past.get_device() == device):
         raise KernelError("step_batch takes tensors of one device")
     n, tokens, table = seq_start.numel(), tok_seq.numel(), pages.shape
     if tok_pos.numel() != tokens or seq_new.numel() != n or seq_past.numel() != n or len(table) != 2 or table[0] != n:
