@@ -685,6 +685,7 @@ __global__ void __launch_bounds__(256) join_q8_kernel(StepBatch sb, AttnQ8 p, in
   const int x = blockIdx.x, y = blockIdx.y, D = p.dim, qpk = p.heads / p.kv_heads;
   const int g = FUSED ? y : y % p.kv_heads, row0 = FUSED ? 0 : y / p.kv_heads * rows_pad;
   const int seq = FUSED ? x : p.tile_seq[x], q0 = FUSED ? 0 : p.tile_q0[x];
+  if (FUSED && sb.seq_new[seq] != 1) return;      // the attention kernel has said so and left no parts; the row may lie past the last
   const int tokens = FUSED ? 1 : min(p.tile_tokens, sb.seq_new[seq] - q0);
   const int n_rows = min(rows_pad, tokens * qpk - row0), quads = D / 4;
   const float* parts = p.parts + (size_t(x) * grid_y + y) * p.teams * size_t(rows_pad) * (D + 2);
