@@ -201,6 +201,9 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
   }
   const int n_blocks = kept_pages + last_pos / KEYS + 1 - kb_lo;
   auto block_of = [&](int i) { return EXTRAS ? (i < kept_pages ? i : kb_lo + i - kept_pages) : i; };   // page i of the walk
+  // its number. Not past the row's end where a table is too narrow for its sequence (steps over a cache in 8 bits, whose pages' reader
+  // has said so): the result is void then, what is read is not.
+  auto page_at = [&](int i) { return pages[EXTRAS ? min(block_of(i), sb.pages_stride - 1) : i]; };
 
   // A warp may be up to three pages ahead of another one (S of page i + 3 is issued after the O += P V of page i, that of page i + 2
   // before P of page i is complete): arrivals for pages i + 1 and i + 2 must not count for page
@@ -235,7 +238,7 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
   // read by the warp's lanes, one each): they are on their way while the other warps fetch Q and tensor
   // memory is allocated. Nobody else touches a barrier before the block-wide barrier below.
   if (TWO && APART ? score_warp : copy_warp) {
-    const int first_pages = lane < n_blocks ? pages[block_of(lane)] : 0;   // lane b: the number of page b
+    const int first_pages = lane < n_blocks ? page_at(lane) : 0;   // lane b: the number of page b
     if (lane == 0) {
       for (int b = 0; b < 3; ++b) {
         mbar_init(bar_s + 8 * b, 1);
@@ -318,7 +321,7 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     if (lane == 0) {
       int asked = min(n_blocks, STAGES);
       for (int b = STAGES; b < n_blocks; ++b) {
-        const int page = pages[block_of(b)];
+        const int page = page_at(b);
         alive = mbar_wait(bar_o + 8 * ((b - STAGES) & 3), ((b - STAGES) >> 2) & 1, error_flag, 6);
         if (!alive) break;
         ask_keys(b, page);
@@ -336,13 +339,13 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     if (lane == 0) {
       int buf = 0, phase = 0;   // S buffer of page i (i % BUFS) and the parity of its barriers ((i / BUFS) & 1)
       if constexpr (APART) {
-        int asked = min(n_blocks, STAGES), next_page = TWO && asked < n_blocks ? pages[block_of(asked)] : 0;
+        int asked = min(n_blocks, STAGES), next_page = TWO && asked < n_blocks ? page_at(asked) : 0;
         for (int i = 0; i < n_blocks; ++i) {
           if (TWO && i > 0 && asked < n_blocks) {      // the stage of page i - 1 is free again when its S is complete
             alive = mbar_wait(bar_s + 8 * ((i - 1) % BUFS), ((i - 1) / BUFS) & 1, error_flag, 6);
             if (!alive) break;
             ask_keys(asked, next_page);
-            if (++asked < n_blocks) next_page = pages[block_of(asked)];
+            if (++asked < n_blocks) next_page = page_at(asked);
           }
           alive = mbar_wait(bar_k + 8 * (i % STAGES), (i / STAGES) & 1, error_flag, 4);
           // S goes where S and P of page i - BUFS were: the O += P V that read that P has completed, and every thread had read
@@ -376,7 +379,7 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
   } else if (value_warp) {
     // ------------------------------------------------------------ O += P V
     if (lane == 0) {
-      int buf = 0, phase = 0, asked = min(n_blocks, STAGES), next_page = TWO && asked < n_blocks ? pages[block_of(asked)] : 0;
+      int buf = 0, phase = 0, asked = min(n_blocks, STAGES), next_page = TWO && asked < n_blocks ? page_at(asked) : 0;
       for (int i = 0; i < n_blocks; ++i) {
         alive = mbar_wait(bar_v + 8 * (i % STAGES), (i / STAGES) & 1, error_flag, 5);
         if (alive) alive = mbar_wait(bar_p + buf * 8, phase, error_flag, 5);
@@ -387,7 +390,7 @@ attention_tc_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
           alive = mbar_wait(bar_o + 8 * ((i - 1) & 3), ((i - 1) >> 2) & 1, error_flag, 6);
           if (!alive) break;
           ask_values(asked, next_page);
-          if (++asked < n_blocks) next_page = pages[block_of(asked)];
+          if (++asked < n_blocks) next_page = page_at(asked);
         }
       }
       if (TWO && !alive)

@@ -2038,13 +2038,14 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
     step = max(1, 1 << max(0, n_pages.bit_length() - 3))
     room = (n_pages + step - 1) // step * step
     k, v = (torch.empty((room, kv_heads, PAGE, wide), dtype=torch.bfloat16, device=device) for _ in range(2))
-    table = torch.empty((batch.n_seqs, batch.pages_stride), dtype=torch.int32, device=device)
+    # entries that unpacking leaves out (a table too narrow, more pages than n_pages: both are said) name a page that there is
+    table = torch.zeros((batch.n_seqs, max(1, batch.pages_stride)), dtype=torch.int32, device=device)
     L, flag, stream = lib(), _flag_at(device.index), _raw_stream(device.index)
     _check(L.ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
                            ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,
                            wide, flag, stream), "attention_q8 (pages)")
     unpacked = StepBatchC.from_buffer_copy(batch)
-    unpacked.pages = table.data_ptr()
+    unpacked.pages, unpacked.pages_stride = table.data_ptr(), table.shape[1]
     if wide != head_dim:
         own, q = q, q.new_empty((n, heads, wide))
         _check(L.ptb_pitch_rows(own.data_ptr(), q.data_ptr(), n * heads, head_dim, wide, stream), "attention_q8 (queries)")

@@ -1,0 +1,42 @@
+"""Prompts over a cache in 8 bits whose steps do not fit their page tables, and workspaces of steps."""
+import pytest
+import torch
+
+from test_q8_gpu import BF, PAGE, Case, K  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def tiles_of(news, tile):
+    tiles = [(b, q0) for b, n in enumerate(news) for q0 in range(0, n, tile)]
+    return [torch.tensor(x, dtype=torch.int32).cuda() for x in zip(*tiles)], len(tiles)
+
+
+@pytest.mark.parametrize("width", [0, 1, 2])
+@pytest.mark.parametrize("kv,qpk,dim,slopes,window", [(1, 2, 64, False, 0), (1, 2, 128, False, 0), (2, 3, 128, True, 0), (1, 2, 64, True, 70), (1, 40, 128, False, 0),
+                                                      (2, 2, 96, False, 0), (1, 2, 256, False, 0)])
+@pytest.mark.parametrize("unpacked", [True, False])
+def test_a_prompt_behind_a_table_too_narrow_is_said(K, kv, qpk, dim, slopes, window, width, unpacked):
+    # sequences of one, two and eight pages behind a table of fewer: nothing past its rows is read, the others' results stand, and the
+    # cache stays as it was
+    c = Case(kv, qpk, dim, [20, 0, 300], [40, 128, 200], slopes=slopes, window=window, seed=3)
+    q, _, _ = c.split()
+    q = q.to(BF)
+    whole = c.table
+    c.append()
+    c.table = whole[:, :width].contiguous()
+    cache, batch = c.device(K)
+    before = [t.clone() for t in cache]
+    lists, n_tiles = tiles_of(c.news, 128)
+    spans = 1 + 2 + 8 - (max(0, 300 - window + 1) // PAGE if window else 0)
+    out = K.attention_q8(q.cuda(), *cache, batch, *lists, n_tiles, 128, c.dev["slopes"], kv, c.scale, window=window, n_pages=spans if unpacked else 0)
+    with pytest.raises(K.KernelError, match="a page that the cache does not have"):
+        K.check_device_errors("cuda")
+    for a, b in zip(cache, before):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    if width:      # the sequence whose pages are all listed
+        c.table = whole
+        want, parts = c.attend(q.float())
+        import plain_q8 as plain
+        got = out.cpu().double().view(want.shape)[:40]
+        assert bool(((got - want[:40]).abs() <= plain.bound(*parts[0])).all())
