@@ -11,7 +11,15 @@
 // the output's own rounding). Sums, maxima and the output are float32. Keys' exponents go into the factor of a page's scores; values'
 // are the unit of the float32 output, which is multiplied by a power of two (exactly) where the unit changes. The unit stays within 2^60
 // of the largest exponent seen, so that the output cannot overflow in small units; smaller pages' weights are scaled instead, which no
-// number notices. The running maximum moves only when a score exceeds it by 2^8 (one vote a tile instead of shuffles for each row).
+// number notices. The running maximum moves only when a score exceeds it by 2^4 (one vote a tile instead of shuffles for each row).
+//
+// A weight's range is float16's: the sum of the weights is float32 and loses none, so a weight too small for float16 would be missing
+// from the output. The largest is therefore at the top, 2^11 to 2^15, and never below 2^5 in a page of values 2^6 below the unit's: 11
+// bits down to 2^-25 of the largest, half a step of 2^-36 below. Beside one key whose score stands out and whose value is zero (an attention
+// sink), the output of 8,191 others is as far off as without it (0.0015 of its norm, the output's own rounding) to the 2^-19 of the
+// weights that they have at 22 to 24 above them; with the largest weight at 1 they lost 0.4 of it at 18 above and all at 20. It costs 0.4 % at
+// the sizes below (a pass of the large batch 181.4 against 180.6 us), and 6 % where a warp has 32 rows, of which one or another moves
+// (chunks of 17 tokens: 54.7 against 51.7); with 2^8 before a maximum moves, and four bits less below it, 181.1 and 52.8.
 //
 // Products. The codes are the larger operand: S^T = K Q^T of 16 keys by 8 rows, O^T = V^T P^T of 16 entries by 8 rows, since few query
 // heads read a K/V head (as the smaller one, four heads of 128 on each K/V head wasted three quarters of the products and twice the
@@ -42,8 +50,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr float MOVE_LOG2 = 8.f;      // float16 weights go up to 2^8 then
-constexpr int UNIT_RANGE = 60, UNIT_SLACK = 3;
+// A weight beside a fresh maximum is 2^WEIGHT_TOP, and float16's largest, 2^15, beside one that has not moved yet.
+constexpr int MOVE_LOG2 = 4, WEIGHT_TOP = 15 - MOVE_LOG2;
+constexpr int UNIT_RANGE = 60, UNIT_SLACK = 6;
 constexpr int MAX_CLUSTER = 8;
 
 struct AttnQ8 {
@@ -410,20 +419,20 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
           }
         }
       }
-      // The unit of the output: that of the tile's values, but for a difference of 2^3 either way, which the weights carry instead (they
-      // stay within float16: 2^8 from the maximum that does not move, 2^3 from here), and for pages 2^60 below the largest.
+      // The unit of the output: that of the tile's values, but where these are smaller by up to 2^6, which the weights carry instead (a
+      // weight of fewer bits then belongs to a smaller value), and for pages 2^60 below the largest.
       bool new_unit = false;
       int far = 0, shift = 0, old_unit = unit;
       if (ev != unit) {
         largest = max(largest, ev);
         const int floor_unit = largest - UNIT_RANGE;
-        new_unit = abs(ev - unit) > UNIT_SLACK && !(ev < floor_unit && unit == floor_unit);
-        if (new_unit) unit = max(ev, floor_unit);
+        new_unit = (ev > unit || ev < unit - UNIT_SLACK) && !(ev < floor_unit && unit == floor_unit);
+        if (new_unit) unit = max(ev > unit ? ev : ev + UNIT_SLACK / 2, floor_unit);
         far = max(ev - unit, -126);
         shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
       }
-      // score - running maximum + shift, in powers of two; a tile that all rows see whole needs no mask
-      const float fk = power_of_two(ek), fshift = float(shift);
+      // score - running maximum + WEIGHT_TOP + shift, in powers of two; a tile that all rows see whole needs no mask
+      const float fk = power_of_two(ek), fshift = float(WEIGHT_TOP + shift);
       const bool whole = key0 + TILE - 1 <= first_pos && (p.window == 0 || key0 > last_pos - p.window);
       float over = -INFINITY;      // by how much the tile exceeds the running maxima
       if (whole && !p.slopes) {
@@ -467,7 +476,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
             over = fmaxf(over, fresh && top != -INFINITY ? INFINITY : top);
           }
       }
-      if (__any_sync(0xffffffffu, over > MOVE_LOG2 + fshift) || new_unit) {
+      if (__any_sync(0xffffffffu, over > float(MOVE_LOG2) + fshift) || new_unit) {
         const float change = power_of_two(min(max(old_unit - unit, -126), 126));
 #pragma unroll
         for (int n = 0; n < NH; ++n)
@@ -498,7 +507,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
           }
       }
       uint32_t pb[NH][ST][2];
-      const float back = power_of_two(-shift);      // the sums are of the weights themselves
+      const float back = power_of_two(-shift);      // the sums are of the weights without it
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
 #pragma unroll
