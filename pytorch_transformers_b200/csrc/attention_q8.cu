@@ -9,9 +9,10 @@
 // Numbers. A code becomes a float16 number exactly (cvt.rn.f16x2.e4m3x2) and meets float16 operands in mma.m16n8k16: queries of 11
 // bits, their row brought to [1, 2) by a power of two, and softmax weights of 11 bits (of bfloat16's 8 they would cost as much as
 // the output's own rounding). Sums, maxima and the output are float32. Keys' exponents go into the factor of a page's scores; values'
-// are the unit of the float32 output, which is multiplied by a power of two (exactly) where the unit changes. The unit stays within 2^60
-// of the largest exponent seen, so that the output cannot overflow in small units; smaller pages' weights are scaled instead, which no
-// number notices. The running maximum moves only when a score exceeds it by 2^4 (one vote a tile instead of shuffles for each row).
+// are the unit of the float32 output, which is multiplied by a power of two (exactly) where the unit changes. The unit is
+// a warp's, for all of its rows, and stays within 2^60 of the largest exponent that it has met, so that the output cannot overflow in
+// small units; products with smaller pages are scaled in float32 before they are added. So a row that does not see (or weigh) the large
+// page keeps the small ones' values, to 2^190 below; smaller ones are lost to it. The running maximum moves only when a score exceeds it by 2^4 (one vote a tile instead of shuffles for each row).
 //
 // A weight's range is float16's: the sum of the weights is float32 and loses none, so a weight too small for float16 would be missing
 // from the output. The largest is therefore at the top, 2^11 to 2^15, and never below 2^5 in a page of values 2^6 below the unit's: 11
@@ -42,6 +43,8 @@
 // 71 heads on one K/V head: 64 sequences of 4,096 keys are slower here than over bfloat16 pages on the tcgen05 kernel (a step of six
 // layers 1.15 against 0.87 ms).
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "q8.cuh"
 #include "tc_common.cuh"
@@ -428,7 +431,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
         const int floor_unit = largest - UNIT_RANGE;
         new_unit = (ev > unit || ev < unit - UNIT_SLACK) && !(ev < floor_unit && unit == floor_unit);
         if (new_unit) unit = max(ev > unit ? ev : ev + UNIT_SLACK / 2, floor_unit);
-        far = max(ev - unit, -126);
+        far = ev - unit;      // 0 to -185
         shift = far < -UNIT_SLACK ? 0 : far;      // 2^shift comes with the exponential
       }
       // score - running maximum + WEIGHT_TOP + shift, in powers of two; a tile that all rows see whole needs no mask
@@ -477,7 +480,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
           }
       }
       if (__any_sync(0xffffffffu, over > float(MOVE_LOG2) + fshift) || new_unit) {
-        const float change = power_of_two(min(max(old_unit - unit, -126), 126));
+        // a unit may rise by 2^245: more than one power of two holds
+        const float change = power_of_two(max((old_unit - unit) / 2, -126)), change2 = power_of_two(max(old_unit - unit - (old_unit - unit) / 2, -126));
 #pragma unroll
         for (int n = 0; n < NH; ++n)
 #pragma unroll
@@ -501,8 +505,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
             const float f = corr * change;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
-              o[n][j][h] *= f;
-              o[n][j][2 + h] *= f;
+              o[n][j][h] = o[n][j][h] * f * change2;
+              o[n][j][2 + h] = o[n][j][2 + h] * f * change2;
             }
           }
       }
@@ -517,12 +521,6 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
           l_run[n][0] = fmaf(s[n][j][0] + s[n][j][2], back, l_run[n][0]);
           l_run[n][1] = fmaf(s[n][j][1] + s[n][j][3], back, l_run[n][1]);
         }
-        if (far != shift) {      // a page 2^60 below the largest: its weights are scaled before they are rounded
-#pragma unroll
-          for (int j = 0; j < ST; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][j][e] *= power_of_two(far);
-        }
 #pragma unroll
         for (int j = 0; j < ST; ++j) {
           pb[n][j][0] = transposed(pack_half(s[n][j][0], s[n][j][1]));
@@ -531,44 +529,62 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
       }
       // output. Keys that no row of the block sees are taken as zero: their codes may be anything.
       const bool edge = key0 + TILE - 1 > last_pos || key0 < low;
+      // apart: a page 2^60 below the largest, whose products are scaled in float32 before they are added. Large batch 185.0 us a pass with this
+      // second copy of the products, 181.0 without; one copy, the sums waiting in local memory: 189.4
+      auto add_values = [&](auto apart) {
 #pragma unroll
-      for (int ks = 0; ks < ST; ++ks)
+        for (int ks = 0; ks < ST; ++ks)
 #pragma unroll
-        for (int rr = 0; rr < VR; ++rr) {
-          uint32_t v[4][VW];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int at = v_at[u & 1] + kt + rr * (PTB_PAGE * 128) + (2 * ks + (u >> 1)) * EIGHT;
-            if (DP == 64) {
-              const uint2 x = *reinterpret_cast<const uint2*>(smem + at);
-              v[u][0] = x.x; v[u][1] = x.y;
-            } else {
-              const uint4 x = *reinterpret_cast<const uint4*>(smem + at);
-              v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
-            }
-          }
-          if (edge) {
+          for (int rr = 0; rr < VR; ++rr) {
+            uint32_t v[4][VW];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-              const int key = key0 + (2 * ks + (u >> 1)) * 8 + kappa<DP>(2 * t4 + (u & 1));
+              const int at = v_at[u & 1] + kt + rr * (PTB_PAGE * 128) + (2 * ks + (u >> 1)) * EIGHT;
+              if (DP == 64) {
+                const uint2 x = *reinterpret_cast<const uint2*>(smem + at);
+                v[u][0] = x.x; v[u][1] = x.y;
+              } else {
+                const uint4 x = *reinterpret_cast<const uint4*>(smem + at);
+                v[u][0] = x.x; v[u][1] = x.y; v[u][VW - 2] = x.z; v[u][VW - 1] = x.w;
+              }
+            }
+            if (edge) {
 #pragma unroll
-              for (int q = 0; q < VW; ++q) v[u][q] = key > last_pos || key < low ? 0u : v[u][q];
+              for (int u = 0; u < 4; ++u) {
+                const int key = key0 + (2 * ks + (u >> 1)) * 8 + kappa<DP>(2 * t4 + (u & 1));
+#pragma unroll
+                for (int q = 0; q < VW; ++q) v[u][q] = key > last_pos || key < low ? 0u : v[u][q];
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < VW; ++q) {
+              uint32_t a[4], b[4];      // entries 4 q, 4 q + 1 and 4 q + 2, 4 q + 3 of the thread's
+              q8_halves(__byte_perm(v[0][q], v[1][q], 0x5140), a[0], a[1]);
+              q8_halves(__byte_perm(v[2][q], v[3][q], 0x5140), a[2], a[3]);
+              q8_halves(__byte_perm(v[0][q], v[1][q], 0x7362), b[0], b[1]);
+              q8_halves(__byte_perm(v[2][q], v[3][q], 0x7362), b[2], b[3]);
+#pragma unroll
+              for (int n = 0; n < NH; ++n) {
+                if constexpr (decltype(apart)::value) {
+                  float x[4] = {}, y[4] = {};
+                  mma_f16(x, a, pb[n][ks][0], pb[n][ks][1]);
+                  mma_f16(y, b, pb[n][ks][0], pb[n][ks][1]);
+                  const float f = power_of_two(max(far, -126)), f2 = power_of_two(min(far + 126, 0));
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    o[n][rr * 8 + q * 2][e] += x[e] * f2 * f;
+                    o[n][rr * 8 + q * 2 + 1][e] += y[e] * f2 * f;
+                  }
+                } else {
+                  mma_f16(o[n][rr * 8 + q * 2], a, pb[n][ks][0], pb[n][ks][1]);
+                  mma_f16(o[n][rr * 8 + q * 2 + 1], b, pb[n][ks][0], pb[n][ks][1]);
+                }
+              }
             }
           }
-#pragma unroll
-          for (int q = 0; q < VW; ++q) {
-            uint32_t a[4], b[4];      // entries 4 q, 4 q + 1 and 4 q + 2, 4 q + 3 of the thread's
-            q8_halves(__byte_perm(v[0][q], v[1][q], 0x5140), a[0], a[1]);
-            q8_halves(__byte_perm(v[2][q], v[3][q], 0x5140), a[2], a[3]);
-            q8_halves(__byte_perm(v[0][q], v[1][q], 0x7362), b[0], b[1]);
-            q8_halves(__byte_perm(v[2][q], v[3][q], 0x7362), b[2], b[3]);
-#pragma unroll
-            for (int n = 0; n < NH; ++n) {
-              mma_f16(o[n][rr * 8 + q * 2], a, pb[n][ks][0], pb[n][ks][1]);
-              mma_f16(o[n][rr * 8 + q * 2 + 1], b, pb[n][ks][0], pb[n][ks][1]);
-            }
-          }
-        }
+      };
+      if (far == shift) add_values(std::false_type{});
+      else add_values(std::true_type{});
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(bar0 + 8 * (MAX_STAGES + st));
@@ -615,7 +631,7 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
       if (r >= n_rows || idle) continue;
       const float2 ml = *reinterpret_cast<const float2*>(merged_ml + 2 * r);
       const bool none = m_run[n][h] == -INFINITY && l_run[n][h] == 0.f;
-      const float share = none ? 0.f : exp2f(m_run[n][h] - ml.x) / ml.y * power_of_two(unit);
+      const float share = none ? 0.f : exp2f(m_run[n][h] - ml.x) / ml.y, in_unit = power_of_two(unit);      // one after the other: their product may be too small a number
       constexpr int COLS = DP == 64 ? 8 : 16;      // entries of a row of the output that a thread holds: [g4][COLS]
       float* to = join + size_t(kg * rows_pad + r) * Shape::PITCH + g4 * COLS;
 #pragma unroll
@@ -624,7 +640,8 @@ attention_q8_kernel(StepBatch sb, AttnQ8 p, const __grid_constant__ CUtensorMap 
         for (int c = 0; c < COLS / 2; c += 2) {
           const float(&x)[4] = o[n][rr * 8 + c], (&y)[4] = o[n][rr * 8 + c + 1];
           *reinterpret_cast<float4*>(to + rr * 128 + 2 * c) =
-              none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x[h] * share, x[2 + h] * share, y[h] * share, y[2 + h] * share);
+              none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                   : make_float4(x[h] * share * in_unit, x[2 + h] * share * in_unit, y[h] * share * in_unit, y[2 + h] * share * in_unit);
         }
     }
   __syncthreads();

@@ -77,3 +77,71 @@ def test_chunks_beside_a_sink(K, kv, qpk, dim, new, tile, above, uneven):
     out = K.attention_q8(q.cuda(), *cache, batch, *lists, n_tiles, tile, None, kv, c.scale, n_splits=1)
     check_positive(c, out, q.float())
     K.check_device_errors("cuda")
+
+
+def pages_of_sizes(kv, qpk, dim, sizes, low):
+    """A sequence of whole pages whose values are about 2^sizes[i], and a token of its own page in ``low``'s size. Keys of pages of another size
+    point away from the queries by hundreds: the weight lies on those of size ``low``."""
+    c = Case(kv, qpk, dim, [PAGE * len(sizes)], [1], seed=len(sizes) + dim)
+    g = torch.Generator().manual_seed(7)
+    n = PAGE * len(sizes)
+    k, v = torch.randn(kv, n, dim, generator=g), torch.randn(kv, n, dim, generator=g)
+    size = torch.tensor(sizes).repeat_interleave(PAGE)
+    v = v.double() * torch.exp2(size.double())[:, None]
+    k[..., 0] = torch.where(size == low, 0.0, -50.0 / c.scale)
+    refill(c, 0, k, v)
+    f = c.fused.view(1, kv, qpk + 2, dim)
+    f[:, :, :qpk, 0] = 8.0
+    f[:, :, qpk, 0] = 0.0
+    f[:, :, qpk + 1] *= 2.0 ** low
+    return c, [i for i, e in enumerate(sizes) if e == low]
+
+
+@pytest.mark.parametrize("kv,qpk,dim", [(1, 1, 64), (2, 3, 128), (1, 20, 128), (1, 71, 64), (1, 9, 256)])
+@pytest.mark.parametrize("sizes", [(20, -70), (-70, 20), (20, -120), (-120, 20), (30, -110, 30, -110), (-110, 30, -30, 30, -110, -110), (-126, 60), (60, -126)])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_small_values_beside_large_ones_without_weight(K, kv, qpk, dim, sizes, splits):
+    low = min(sizes)
+    c, seen = pages_of_sizes(kv, qpk, dim, sizes, low)
+    cache, batch = c.device(K)
+    out = K.attention_decode_q8(c.dev["fused"], *cache, batch, None, None, kv, qpk, dim, c.scale, n_splits=splits)
+    c.append()
+    # the other pages' weights are e^-300 and less: the output is that of the seen pages and the new token's
+    ids = c.table[0, seen + [len(sizes)]].long()
+    k, v = (plain.values(c.codes[x], c.exps[x])[ids].transpose(1, 2).reshape(-1, kv, dim)[:PAGE * len(seen) + 1] for x in "kv")
+    want, most, size = plain.attend(c.split()[0], k, v, c.scale, torch.tensor([PAGE * len(seen)]))
+    over = (out.cpu().double().view(want.shape) - want).abs() - plain.bound(want, most, size, k.shape[0]) - 2.0 ** -134      # bfloat16's last place
+    assert float(most.max()) < 2.0 ** (low + 4) and float(over.max()) <= 0
+    K.check_device_errors("cuda")
+
+
+@pytest.mark.parametrize("kv,qpk,dim", [(1, 2, 64), (2, 1, 128), (1, 2, 256), (1, 5, 80)])
+@pytest.mark.parametrize("sizes,window", [((-70, 20), 0), ((-120, 20), 0), ((20, -70, -70), 64), ((20, -120, -120), 64), ((-120, 20, -110, -110), 64)])
+@pytest.mark.parametrize("tile", [64, 128])
+def test_rows_that_do_not_see_the_large_values(K, kv, qpk, dim, sizes, window, tile):
+    # hidden by the causal order, or left of the window: rows of one tile beside others that see them
+    n = PAGE * len(sizes)
+    c = Case(kv, qpk, dim, [0], [n], window=window, seed=dim)
+    f = c.fused.view(n, kv, qpk + 2, dim)
+    f[:, :, qpk + 1] *= torch.exp2(torch.tensor(sizes).repeat_interleave(PAGE).float())[:, None, None]
+    q = c.split()[0].to(BF)
+    c.append()
+    cache, batch = c.device(K)
+    lists, n_tiles = tiles_of(c.news, tile)
+    out = K.attention_q8(q.cuda(), *cache, batch, *lists, n_tiles, tile, None, kv, c.scale, window=window)
+    c.check(out, q.float())
+    K.check_device_errors("cuda")
+
+
+@pytest.mark.parametrize("e", [-126, -118, -100])
+@pytest.mark.parametrize("splits", [1, 3, 16])
+def test_the_smallest_values(K, e, splits):
+    c = Case(2, 3, 64, [1000], [1], seed=1)
+    c.exps["v"][:] = e
+    c.fused.view(1, 2, 5, 64)[:, :, 4] *= 2.0 ** e
+    cache, batch = c.device(K)
+    out = K.attention_decode_q8(c.dev["fused"], *cache, batch, None, None, 2, 3, 64, c.scale, n_splits=splits)
+    c.append()
+    want, parts = c.attend(c.split()[0])
+    over = (out.cpu().double().view(want.shape) - want).abs() - plain.bound(*parts[0]) - 2.0 ** -134
+    assert float(over.max()) <= 0 and bool((out != 0).any())
