@@ -571,9 +571,8 @@ PTB_API int ptb_attention_decode_tc(const void* fused, void* k_pool, void* v_poo
   if (pool_pages <= 0 || ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool) |
                            reinterpret_cast<uintptr_t>(fused)) & 15))
     return PTB_ERR_ALIGN;
-  const CUtensorMap* km = pool_map(k_pool, pool_pages, kv_heads, DD);
-  const CUtensorMap* vm = pool_map(v_pool, pool_pages, kv_heads, DD);
-  if (km == nullptr || vm == nullptr) return PTB_ERR_LAUNCH;
+  CUtensorMap km, vm;
+  if (!pool_map(&km, k_pool, pool_pages, kv_heads, DD) || !pool_map(&vm, v_pool, pool_pages, kv_heads, DD)) return PTB_ERR_LAUNCH;
   DecodeTcParams p;
   p.heads = heads; p.kv_heads = kv_heads; p.n_splits = n_splits; p.n_teams = n_teams; p.rot_pairs = rot_pairs;
   p.write_cache = write_cache; p.scale = scale; p.interleaved = interleaved ? 1 : 0;
@@ -592,7 +591,7 @@ PTB_API int ptb_attention_decode_tc(const void* fused, void* k_pool, void* v_poo
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, attention_decode_tc_kernel, (const __nv_bfloat16*)fused, (__nv_bfloat16*)k_pool,
-                         (__nv_bfloat16*)v_pool, (__nv_bfloat16*)out, *sb, rope_cos, rope_sin, p, *km, *vm,
+                         (__nv_bfloat16*)v_pool, (__nv_bfloat16*)out, *sb, rope_cos, rope_sin, p, km, vm,
                          team_parts, tickets, error_flag) != cudaSuccess) {
     (void)cudaGetLastError();
     return PTB_ERR_LAUNCH;

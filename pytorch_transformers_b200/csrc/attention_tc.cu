@@ -962,16 +962,15 @@ template <int D, bool BIAS>
 int launch_tc_pair(const void* q, const void* k_pool, const void* v_pool, int pool_pages, void* out, const StepBatch& sb,
                    const int* tile_seq, const int* tile_q0, int n_tiles, const TcParams& p, int* error_flag,
                    cudaStream_t stream) {
-  const CUtensorMap* km = pool_map(k_pool, pool_pages, p.kv_heads, D);
-  const CUtensorMap* vm = pool_map(v_pool, pool_pages, p.kv_heads, D);
-  if (km == nullptr || vm == nullptr) return PTB_ERR_LAUNCH;
+  CUtensorMap km, vm;
+  if (!pool_map(&km, k_pool, pool_pages, p.kv_heads, D) || !pool_map(&vm, v_pool, pool_pages, p.kv_heads, D)) return PTB_ERR_LAUNCH;
   constexpr size_t smem = PairShape<D>::SMEM;
   static SharedLimit limit;
   if (!limit.allows(attention_tc_pair_kernel<D, BIAS>, smem)) return PTB_ERR_LAUNCH;
   const int qpk = p.heads / p.kv_heads;
   dim3 grid(p.kv_heads * ((qpk + 1) / 2), n_tiles);
   attention_tc_pair_kernel<D, BIAS><<<grid, PAIR_THREADS, smem, stream>>>(
-      (const __nv_bfloat16*)q, (__nv_bfloat16*)out, sb, tile_seq, tile_q0, p, *km, *vm, error_flag);
+      (const __nv_bfloat16*)q, (__nv_bfloat16*)out, sb, tile_seq, tile_q0, p, km, vm, error_flag);
   return launch_status();
 }
 }  // namespace
@@ -986,6 +985,8 @@ PTB_API int ptb_attention_tc_supports_sizes(int head_dim, int v_dim) {
   return ((head_dim == 64 || head_dim == 128) && v_dim == head_dim) || (head_dim == 192 && v_dim == 128) ? 1 : 0;
 }
 PTB_API int ptb_attention_tc_tile_tokens() { return TQ; }
+// for tests: descriptions of pools that the library holds, at most POOL_MAPS
+PTB_API int ptb_pool_maps() { return pool_maps_kept().load(); }
 
 namespace {
 template <int DK, int DV, bool BIAS, bool WIDE, bool EXTRAS = false, bool TWO = false, bool SHORT = false>
@@ -1006,16 +1007,15 @@ int launch_tc(const void* q, const void* k_pool, const void* v_pool, int pool_pa
         return launch_tc<DK, DV, BIAS, WIDE, EXTRAS, true, SHORT>(q, k_pool, v_pool, pool_pages, out, sb, tile_seq, tile_q0, n_tiles, p,
                                                                   error_flag, stream);
     }
-    const CUtensorMap* km = pool_map(k_pool, pool_pages, p.kv_heads, DK);
-    const CUtensorMap* vm = pool_map(v_pool, pool_pages, p.kv_heads, DV);
-    if (km == nullptr || vm == nullptr) return PTB_ERR_LAUNCH;
+    CUtensorMap km, vm;
+    if (!pool_map(&km, k_pool, pool_pages, p.kv_heads, DK) || !pool_map(&vm, v_pool, pool_pages, p.kv_heads, DV)) return PTB_ERR_LAUNCH;
     const size_t smem = 1024 + TQ * DK * 2 + TcShape<TWO>::STAGES * KEYS * (DK + DV) * 2 + 192;
     static SharedLimit limit;
     if (!limit.allows(attention_tc_kernel<DK, DV, BIAS, WIDE, EXTRAS, TWO, SHORT>, smem)) return PTB_ERR_LAUNCH;
     dim3 grid(p.heads, n_tiles);
     attention_tc_kernel<DK, DV, BIAS, WIDE, EXTRAS, TWO, SHORT><<<grid, TcThreads<DK, WIDE, EXTRAS, TWO, SHORT>::BLOCK, smem, stream>>>(
         (const __nv_bfloat16*)q, (const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, (__nv_bfloat16*)out, sb,
-        tile_seq, tile_q0, p, *km, *vm, error_flag);
+        tile_seq, tile_q0, p, km, vm, error_flag);
   }
   return launch_status();
 }

@@ -5,9 +5,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <map>
+#include <atomic>
 #include <mutex>
-#include <tuple>
 
 #include "mma_common.cuh"
 
@@ -238,13 +237,19 @@ template <> __device__ __forceinline__ void tmem_st_u32<32>(uint32_t taddr, cons
 
 // ---- host side
 // a pool of one cache entry, [pages][kv_heads][64 keys][D], seen as rows of D values: boxes of 64 keys x
-// 64 dims land in the 128-byte-swizzle layout. Pools do not move: a map per pool is made once and kept.
-inline const CUtensorMap* pool_map(const void* pool, int pool_pages, int kv_heads, int d) {
-  struct Key {
-    const void* p; long long rows; int d;
-    bool operator<(const Key& o) const { return std::tie(p, rows, d) < std::tie(o.p, o.rows, o.d); }
+// 64 dims land in the 128-byte-swizzle layout. Most pools stay where they are, and their maps are kept; workspaces and the
+// storage of a cache that changes its size come and go, so a map has one place to be kept in, by its address and sizes, and gives way to the next
+// one that belongs there. A map says nothing of what the memory holds: one that is found is right.
+constexpr int POOL_MAPS = 2048;
+inline std::atomic<int>& pool_maps_kept() {
+  static std::atomic<int> n{0};
+  return n;
+}
+inline bool pool_map(CUtensorMap* map, const void* pool, int pool_pages, int kv_heads, int d) {
+  struct Kept {
+    const void* p; long long rows; int d; CUtensorMap map;
   };
-  static std::map<Key, CUtensorMap> cache;
+  static Kept kept[POOL_MAPS];
   static std::mutex mu;
   static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
   std::lock_guard<std::mutex> lock(mu);
@@ -253,21 +258,27 @@ inline const CUtensorMap* pool_map(const void* pool, int pool_pages, int kv_head
     cudaDriverEntryPointQueryResult qr;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) != cudaSuccess ||
         qr != cudaDriverEntryPointSuccess)
-      return nullptr;
+      return false;
     encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   }
-  const Key key{pool, (long long)pool_pages * kv_heads * KEYS, d};
-  auto it = cache.find(key);
-  if (it != cache.end()) return &it->second;
-  CUtensorMap m;
-  const cuuint64_t dims[2] = {cuuint64_t(d), cuuint64_t(key.rows)};
-  const cuuint64_t strides[1] = {cuuint64_t(d) * 2};
-  const cuuint32_t box[2] = {64, cuuint32_t(KEYS)};
-  const cuuint32_t elem[2] = {1, 1};
-  if (encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return nullptr;
-  return &cache.emplace(key, m).first->second;
+  const long long rows = (long long)pool_pages * kv_heads * KEYS;
+  // addresses are multiples of 512 for what the allocator gives out, of 16 at least; entries of one cache lie a multiple of pages apart
+  const unsigned long long mixed = ((unsigned long long)(uintptr_t)pool / 16 + (unsigned long long)rows * 131 + d) * 0x9e3779b97f4a7c15ull;
+  Kept& k = kept[mixed >> 53];      // 11 bits: POOL_MAPS
+  if (k.p != pool || k.rows != rows || k.d != d) {
+    const cuuint64_t dims[2] = {cuuint64_t(d), cuuint64_t(rows)};
+    const cuuint64_t strides[1] = {cuuint64_t(d) * 2};
+    const cuuint32_t box[2] = {64, cuuint32_t(KEYS)};
+    const cuuint32_t elem[2] = {1, 1};
+    CUtensorMap m;
+    if (encode(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+    if (k.p == nullptr) pool_maps_kept() += 1;
+    k.p = pool; k.rows = rows; k.d = d; k.map = m;
+  }
+  *map = k.map;
+  return true;
 }
 

@@ -40,3 +40,22 @@ def test_a_prompt_behind_a_table_too_narrow_is_said(K, kv, qpk, dim, slopes, win
         import plain_q8 as plain
         got = out.cpu().double().view(want.shape)[:40]
         assert bool(((got - want[:40]).abs() <= plain.bound(*parts[0])).all())
+
+
+def test_descriptions_of_pools_that_come_and_go_are_not_kept_for_good(K):
+    # the same pages as pools of 2,500 sizes: two descriptions each
+    L = K.lib()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(2600, 1, PAGE, 64, generator=g, device="cuda", dtype=BF) for _ in "kv")
+    q = torch.randn(130, 2, 64, generator=g, device="cuda", dtype=BF)
+    ints = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([0] * 130, list(range(130)), [0], [130], [0])]
+    batch = K.step_batch(*ints, torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda())
+    lists, n_tiles = tiles_of([130], 128)
+    def run(pages):
+        return K.attention_tc_extras(q, k[:pages], v[:pages], batch, *lists, n_tiles, 1, 0.125)
+    first = run(3)
+    for pages in range(4, 2504):
+        run(pages)
+    assert 0 < L.ptb_pool_maps() <= 2048
+    assert torch.equal(run(3), first) and torch.equal(run(1000), first)
+    K.check_device_errors("cuda")
