@@ -1845,7 +1845,8 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
                pages: torch.Tensor) -> StepBatchC:
     """The description of a step for the kernels from int32 tensors on the device (``StepContext`` builds it for the engine):
     sequence and position of every token, each sequence's first token, tokens of this step and tokens before it, and the page
-    table [sequences, width], wide enough for every sequence's tokens. The tensors must outlive the kernels that read them."""
+    table [sequences, width], wide enough for every sequence's tokens. The description holds the tensors: it must outlive the calls that
+    take it, and on another stream than the tensors' own the kernels that read them."""
     for t in (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages):
         if not (t.dtype is torch.int32 and t.is_cuda and t.is_contiguous()):
             raise KernelError("step_batch takes contiguous int32 tensors on the device")
@@ -1857,7 +1858,7 @@ def step_batch(tok_seq: torch.Tensor, tok_pos: torch.Tensor, seq_start: torch.Te
         raise KernelError("step_batch: the arrays' lengths do not fit one another")
     batch = StepBatchC(tok_seq.data_ptr(), tok_pos.data_ptr(), seq_start.data_ptr(), seq_new.data_ptr(), seq_past.data_ptr(),
                        pages.data_ptr(), table[1], tokens, n)
-    batch.device = device
+    batch.device, batch.tensors = device, (tok_seq, tok_pos, seq_start, seq_new, seq_past, pages)
     return batch
 
 
