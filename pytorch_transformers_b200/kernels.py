@@ -1994,7 +1994,8 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     """Causal attention of prompts and chunks over a cache in 8 bits that holds their keys and values already. ``q`` [tokens, heads,
     head_dim] bfloat16; tiles of ``tile_tokens`` consecutive new tokens as for the other prompt kernels. ``n_pages``: the pages that the
     step's sequences span (their sum, or more): where it is given, steps in tiles of 128 tokens with heads of up to 128 take their
-    pages as bfloat16 values into a workspace once and run the tcgen05 prompt kernel on it. ``n_splits``: as ``attention_decode_q8``
+    pages as bfloat16 values into a workspace once (twice their codes' bytes) and run the tcgen05 prompt kernel on it. Steps whose tiles
+    hold few tokens, and those for whose workspace the device has no room, read the codes as all others do. ``n_splits``: as ``attention_decode_q8``
     takes it, for the others. A value held as no number reaches the rows of a tile that share its matrix instructions, whether they see
     it or not (single tokens: the rows that see it). Returns [tokens, heads * head_dim]."""
     what = "attention_q8"
@@ -2010,9 +2011,11 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     for t in (tile_seq, tile_q0):
         if not (t.dtype is torch.int32 and t.numel() >= n_tiles and t.get_device() == device and t.is_contiguous()):
             raise KernelError(f"{what}: tile lists must be contiguous int32 tensors of {n_tiles} tiles on the queries' device")
-    if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and head_dim <= 128:
-        return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
-                                      window, n_pages)
+    if n_pages > 0 and tile_tokens == TC_TILE_TOKENS and head_dim <= 128 and n >= Q8_UNPACK_TILE_TOKENS * n_tiles:
+        workspace = _unpacked_pages(n_pages, kv_heads, head_dim, q.device)
+        if workspace is not None:
+            return _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale,
+                                          window, n_pages, workspace)
     if n_splits > 8:
         n_splits = n_splits // 8 * 8
     pages = batch.pages_stride if n_pages <= 0 else min(batch.pages_stride, n_pages)
@@ -2032,13 +2035,29 @@ def attention_q8(q: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_p
     return out
 
 
-def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale, window, n_pages):
+# Tokens that a tile of 128 holds on average from which a step's pages are unpacked. One sequence that brings a prompt beside 63 that bring
+# a token each unpacks all of their pages for little: 512 tokens beside 1,024 past, 32 heads of 128 on 8 K/V heads (8.6 tokens a
+# tile) 310 us and 274 MB of workspace against 269 from the codes, 71 of 64 on 1 409 against 140; 1,024 beside 8,192 (15.3) 2,081 us and 2 GB
+# against 1,931, 2,807 against 1,013. Tiles that are full: 512 tokens after 8,192 157 us against 347, 158 against 404; half full (129 tokens in
+# two tiles, eight sequences) 462 against 973, 622 against 766.
+Q8_UNPACK_TILE_TOKENS = 32
+
+
+def _unpacked_pages(n_pages: int, kv_heads: int, head_dim: int, device):
+    """Room for pages of keys and values as bfloat16 (heads of other sizes as heads of 64 or 128, with zeros), or None where the device has none:
+    a cache in 8 bits may fill it."""
+    wide = 64 if head_dim <= 64 else 128
+    try:
+        return tuple(torch.empty((n_pages, kv_heads, PAGE, wide), dtype=torch.bfloat16, device=device) for _ in range(2))
+    except torch.OutOfMemoryError:
+        return None
+
+
+def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, tile_q0, n_tiles, slopes, kv_heads, scale, window, n_pages,
+                           workspace):
     n, heads, head_dim = q.shape
-    device, wide = q.device, 64 if head_dim <= 64 else 128      # heads of other sizes as heads of these, with zeros
-    # sizes in steps of an eighth: the prompt kernel keeps a tensor map for every size of pool
-    step = max(1, 1 << max(0, n_pages.bit_length() - 3))
-    room = (n_pages + step - 1) // step * step
-    k, v = (torch.empty((room, kv_heads, PAGE, wide), dtype=torch.bfloat16, device=device) for _ in range(2))
+    k, v = workspace
+    device, wide = q.device, k.shape[-1]
     # entries that unpacking leaves out (a table too narrow, more pages than n_pages: both are said) name a page that there is
     table = torch.zeros((batch.n_seqs, max(1, batch.pages_stride)), dtype=torch.int32, device=device)
     L, flag, stream = lib(), _flag_at(device.index), _raw_stream(device.index)
@@ -2054,7 +2073,7 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
         out = attention_tc_extras(q, k, v, unpacked, tile_seq, tile_q0, n_tiles, kv_heads, scale, window=window)
     else:
         out = q.new_empty((n, heads * wide))
-        _check(L.ptb_attention_tc_extras_biased(q.data_ptr(), k.data_ptr(), v.data_ptr(), room, out.data_ptr(), ctypes.byref(unpacked),
+        _check(L.ptb_attention_tc_extras_biased(q.data_ptr(), k.data_ptr(), v.data_ptr(), n_pages, out.data_ptr(), ctypes.byref(unpacked),
                                                 tile_seq.data_ptr(), tile_q0.data_ptr(), n_tiles, slopes.data_ptr(), heads, kv_heads,
                                                 wide, scale, window, flag, stream), "attention_q8 (prompt)")
     if wide != head_dim:

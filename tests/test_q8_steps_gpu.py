@@ -59,3 +59,61 @@ def test_descriptions_of_pools_that_come_and_go_are_not_kept_for_good(K):
     assert 0 < L.ptb_pool_maps() <= 2048
     assert torch.equal(run(3), first) and torch.equal(run(1000), first)
     K.check_device_errors("cuda")
+
+
+def long_cache(K, kv, dim, tokens, seqs):
+    """Pages of ``seqs`` sequences of ``tokens`` tokens, made on the device."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    per = (tokens + PAGE - 1) // PAGE
+    cache = []
+    for _ in "kv":
+        cache += [torch.randn(seqs * per, kv, PAGE, dim, generator=g, device="cuda", dtype=BF).to(K.Q8), torch.zeros(seqs * per, kv, dtype=torch.int8, device="cuda")]
+    return cache, torch.arange(seqs * per, dtype=torch.int32).view(seqs, per)
+
+
+def described(K, table, pasts, news):
+    ints = [torch.tensor(x, dtype=torch.int32).cuda() for x in ([b for b, n in enumerate(news) for _ in range(n)],
+                                                                [p + i for p, n in zip(pasts, news) for i in range(n)],
+                                                                [sum(news[:b]) for b in range(len(news))], news, pasts)]
+    return K.step_batch(*ints, table.cuda())
+
+
+def test_a_prompt_beside_single_tokens_takes_no_workspace(K):
+    # one of 32 sequences of 2,048 tokens brings 200, the others one each: their pages as bfloat16 values would be 268 MB
+    pasts, news = [1800] + [2000] * 31, [200] + [1] * 31
+    cache, table = long_cache(K, 8, 128, 2048, 32)
+    batch = described(K, table, pasts, news)
+    lists, n_tiles = tiles_of(news, 128)
+    q = torch.randn(sum(news), 16, 128, device="cuda", dtype=BF)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1, n_pages=32 * 32)
+    assert torch.cuda.max_memory_allocated() - before < 64 << 20
+    assert torch.equal(out, K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1))
+    K.check_device_errors("cuda")
+
+
+def test_a_prompt_without_room_for_a_workspace_reads_the_codes(K):
+    # 300 tokens after 60,000: pages of 247 MB as bfloat16 values, on a device that the process may not use more of
+    cache, table = long_cache(K, 8, 128, 60300, 1)
+    batch = described(K, table, [60000], [300])
+    lists, n_tiles = tiles_of([300], 128)
+    q = torch.randn(300, 16, 128, device="cuda", dtype=BF)
+    want = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1)
+    pages = cache[0].shape[0]
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            torch.empty(pages, 8, PAGE, 128, dtype=BF, device="cuda")
+        out = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1, n_pages=pages)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.equal(out, want)
+    K.check_device_errors("cuda")
+    unpacked = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1, n_pages=pages)
+    # each off by its rounding (2^-8) and by weights of 11 bits beside values up to 5.5 (2^-11 of them)
+    torch.testing.assert_close(unpacked.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
