@@ -166,9 +166,8 @@ class PreTrainedCausalLM(CausalLM):
     def _ensure_cache(self, max_tokens: int, kv_dtype: Optional[torch.dtype] = None) -> Cache:
         cache = getattr(self, "_cache", None)
         if cache is None or cache.max_tokens < max_tokens or cache.records or cache.kv_dtype != kv_dtype:
-            if cache is not None and cache.records:
-                cache = None  # somebody holds sequences in it: leave it alone, use a private one
-            self._cache = None
+            # given up before the next one is allocated: both may not fit. One in which somebody holds sequences stays theirs
+            self._cache = cache = None
             cache = self.new_cache(max_tokens, kv_dtype=kv_dtype)
             self._cache = cache
         return cache
