@@ -76,6 +76,24 @@ class GenerateOutput:
     finish_reasons: Optional[List[str]] = None
 
 
+def _cache_tokens(prompts, budget: int, max_batch: int, same_as=None) -> int:
+    """Tokens of cache, in whole pages, of the largest batch: each request's final length, rounded up to pages; requests of a batch with
+    the same prompt (``same_as``: as ``run_generation`` takes it) share its whole pages and have one of their own at least."""
+    need = 0
+    for i in range(0, len(prompts), max_batch):
+        pages, seen = 0, set()
+        for r in range(i, min(i + max_batch, len(prompts))):
+            n = len(prompts[r])
+            own = (n + budget + PAGE - 1) // PAGE
+            if same_as is not None:
+                if same_as[r] in seen:
+                    own = max(1, own - n // PAGE)
+                seen.add(same_as[r])
+            pages += own
+        need = max(need, pages * PAGE)
+    return need
+
+
 class _CacheStepper:
     """The generation loop's view of a model and a cache. Prompts that together exceed
     ``max_step_tokens`` are fed in several steps (whole prompts grouped, a longer prompt cut into
@@ -219,11 +237,8 @@ class PreTrainedCausalLM(CausalLM):
         budget = opts.new_token_budget(padded_len if tensor_in else longest,
                                        getattr(self.config, "max_position_embeddings", None))
         max_batch = max(1, min(int(max_batch_size), len(expanded)))
-        # the largest batch decides the cache: each request's final length, rounded up to whole pages
-        need = 0
-        for i in range(0, len(expanded), max_batch):
-            need = max(need, sum((len(p) + budget + PAGE - 1) // PAGE * PAGE for p in expanded[i:i + max_batch]))
-        cache = self._ensure_cache(need, kv_dtype)
+        same_as = [i - i % n_ret for i in range(len(expanded))] if share_prompts and n_ret > 1 else None
+        cache = self._ensure_cache(_cache_tokens(expanded, budget, max_batch, same_as), kv_dtype)
         selector = DeviceSelector(self.build.kernels, self.device, self.spec.vocab_size, opts, max_rows=max_batch,
                                   max_history=longest + budget)
 
@@ -253,7 +268,7 @@ class PreTrainedCausalLM(CausalLM):
         results = run_generation(_CacheStepper(self, cache, max_step_tokens), selector, expanded, opts, budget, max_batch,
                                  on_token=_on_token if on_token is not None else None,
                                  keep_logits=opts.output_logits, on_step=_on_step if stream_steps else None,
-                                 same_as=[i - i % n_ret for i in range(len(expanded))] if share_prompts and n_ret > 1 else None)
+                                 same_as=same_as)
         self.check_errors()
         if streamer is not None:
             if not stream_steps:

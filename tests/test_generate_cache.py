@@ -35,3 +35,62 @@ def test_a_cache_with_open_sequences_is_left_to_its_holder(model):
     slot = cache.open()
     assert model._ensure_cache(64) is not cache
     assert slot in cache.records
+
+
+class BookkeepingStepper:
+    """A model's steps as far as the cache notices them."""
+
+    def __init__(self, cache):
+        self.cache, self.peak = cache, 0
+
+    def open(self):
+        return self.cache.open()
+
+    def close(self, slot):
+        self.cache.close(slot)
+
+    def fork(self, slot):
+        return self.cache.fork(slot)
+
+    def step(self, slots, token_lists):
+        for slot, tokens in zip(slots, token_lists):
+            self.cache.reserve(slot, len(tokens))
+        for slot, tokens in zip(slots, token_lists):
+            self.cache.commit(slot, len(tokens))
+        self.cache.check()
+        self.peak = max(self.peak, self.cache.groups[0].pool.in_use)
+        return torch.zeros(len(slots), 7)
+
+
+@pytest.mark.parametrize("max_batch", [1, 2, 3, 8, 40])
+@pytest.mark.parametrize("n_ret", [1, 2, 5])
+@pytest.mark.parametrize("lengths,budget", [([1], 1), ([64], 1), ([63, 64, 65], 70), ([200, 3], 64), ([640], 129), ([5, 1000, 128], 3)])
+def test_shared_prompts_ask_for_their_pages_once(model, lengths, budget, n_ret, max_batch):
+    from pytorch_transformers_b200.config import GenerationConfig
+    from pytorch_transformers_b200.engine import run_generation
+    from pytorch_transformers_b200.modeling import _cache_tokens
+    from test_generation_loop import ArgmaxSelector
+    prompts = [[3] * n for n in lengths for _ in range(n_ret)]
+    max_batch = min(max_batch, len(prompts))
+    same_as = [i - i % n_ret for i in range(len(prompts))] if n_ret > 1 else None
+    need = _cache_tokens(prompts, budget, max_batch, same_as)
+    stepper = BookkeepingStepper(model.new_cache(need))
+    results = run_generation(stepper, ArgmaxSelector(), prompts, GenerationConfig(), budget, max_batch, same_as=same_as)
+    assert [len(r.tokens) for r in results] == [budget] * len(prompts)
+    # tight but for the page of the last token, which is chosen and not run
+    assert need // 64 - max_batch <= stepper.peak <= need // 64
+    if n_ret > 1 and max_batch >= n_ret and max(lengths) >= 128:
+        assert need < _cache_tokens(prompts, budget, max_batch)
+
+
+def test_generate_asks_for_that_much(model, monkeypatch):
+    asked = []
+
+    def ensure(tokens, kv_dtype=None):
+        asked.append(tokens)
+        raise KeyboardInterrupt
+    monkeypatch.setattr(model, "_ensure_cache", ensure)
+    for share in (False, True):
+        with pytest.raises(KeyboardInterrupt):
+            model.generate([[3] * 100], max_new_tokens=20, num_return_sequences=4, do_sample=True, share_prompts=share)
+    assert asked == [4 * 128, 128 + 3 * 64]
