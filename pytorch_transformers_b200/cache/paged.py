@@ -114,8 +114,17 @@ class StorageGroup:
         fresh = self._storage(num_pages) if num_pages >= len(held) else ()     # allocated before anything changes
         moved = self.pool.renumber(num_pages)
         self.copy_pages(held, [moved.get(i, i) for i in held], out=[t for t in fresh if t is not None and t.numel()])
+        _read_by_this_stream(self.tensors())
         self.k, self.v, self.k_exp, self.v_exp = fresh
         return moved
+
+
+def _read_by_this_stream(tensors) -> None:
+    """Storage about to be given up may be on its way to other storage on another stream than the one it was allocated on: its memory is
+    nobody else's until the copy has read it."""
+    for t in tensors:
+        if t.is_cuda:
+            t.record_stream(torch.cuda.current_stream(t.device))
 
 
 class Cache:
@@ -320,6 +329,7 @@ class Cache:
         if self._slots_by_pages and slots > self.max_slots:
             state = torch.zeros((slots, self.state_width), dtype=torch.float32, device=self.device)
             state[:self.max_slots] = self.state
+            _read_by_this_stream([self.state])
             self.state, self.max_slots = state, slots
             self.slots.grow(slots)
 
