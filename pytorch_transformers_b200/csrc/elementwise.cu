@@ -680,3 +680,10 @@ PTB_API int ptb_glu_act(int dtype, const void* in, void* out, int rows, int f, i
     return PTB_ERR_DTYPE;
   return launch_status();
 }
+
+// What this thread may do while a stream is being captured (cudaStreamCaptureMode: 0 global, 1 thread-local, 2 relaxed); returns what it was.
+PTB_API int ptb_capture_mode(int mode) {
+  cudaStreamCaptureMode m = cudaStreamCaptureMode(mode);
+  if (cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess) (void)cudaGetLastError();
+  return int(m);
+}

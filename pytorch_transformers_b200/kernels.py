@@ -521,7 +521,19 @@ def error_flag(device) -> torch.Tensor:
         device = _with_index(device)
         flag = _error_flags.get(device)
         if flag is None:
-            flag = _error_flags[device] = torch.zeros(1, dtype=torch.int32, device=device)
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                # beside the capture: it would take the zeroing along, and every replay erase what other kernels have raised
+                side, L = torch.cuda.Stream(device), lib()
+                mode = L.ptb_capture_mode(2)      # relaxed: this thread may wait for another stream meanwhile
+                try:
+                    with torch.cuda.stream(side):
+                        flag = torch.zeros(1, dtype=torch.int32, device=device)
+                    side.synchronize()
+                finally:
+                    L.ptb_capture_mode(mode)
+            else:
+                flag = torch.zeros(1, dtype=torch.int32, device=device)
+            _error_flags[device] = flag
     return flag
 
 
