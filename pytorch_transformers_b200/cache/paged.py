@@ -263,7 +263,8 @@ class Cache:
             g.copy_pages([pages[i] for i in places], own)
             for i, p in zip(places, own):
                 pages[i] = p
-            g.pool.share(p for i, p in enumerate(pages) if p >= 0 and i not in places)
+            copied = set(places)
+            g.pool.share(p for i, p in enumerate(pages) if p >= 0 and i not in copied)
             copy.pages[gi] = pages
         if self.state_width:
             self.state[new].copy_(self.state[slot])
