@@ -2094,6 +2094,16 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
     return out
 
 
+def _page_numbers(pages) -> np.ndarray:
+    """``pages`` in 32 bits. What has another value there (numbers past 32 bits, fractions) is refused."""
+    a = np.asarray(pages)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() >= 1 << 31):
+            raise KernelError(f"copy_pages takes page numbers, got {a.dtype} from {a.min()} to {a.max()}")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
+
+
 def copy_pages(pools, src, dst, out=None):
     """Pages ``src[i]`` to ``dst[i]`` in every tensor of ``pools`` ([entries, pages, ...], contiguous, of any type; at most eight),
     or into the tensors ``out`` of the same types and page shapes (other storage, with pages of its own number). ``src`` and ``dst``:
@@ -2101,7 +2111,7 @@ def copy_pages(pools, src, dst, out=None):
     may be both. One launch for up to 960 pairs. Returns the tensors written to."""
     pools = list(pools)
     into = pools if out is None else list(out)
-    src, dst = np.ascontiguousarray(src, dtype=np.int32), np.ascontiguousarray(dst, dtype=np.int32)
+    src, dst = _page_numbers(src), _page_numbers(dst)
     k = len(pools)
     if not (0 < k <= 8 and len(into) == k and src.ndim == 1 and src.shape == dst.shape):
         raise KernelError("copy_pages takes one to eight tensors, as many targets and one target page for each source page")
