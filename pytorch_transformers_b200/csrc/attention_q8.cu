@@ -848,10 +848,15 @@ bool known(int heads, int kv_heads, int dim, int pool_pages) {
 }
 // Blocks that share a row's pages: as many as the SMs take at a time, two pages each at least. Up to eight form a cluster and join
 // through its shared memory; more are a multiple of eight, of eight pages each at least, whose clusters join through a workspace.
-int splits_of(long long blocks, int pages, int dp, int nh) {
-  const long long slots = (nh >= 4 || dp == 256 ? 1ll : 2ll) * sm_count();
+// `beside` a weight stream on another branch of a graph the blocks' shared memory keeps the stream's blocks off their SMs, and they are as many as half
+// of the SMs at most, below eight a power of two for each row's pages. Six layers of 32 heads of 128 on 8, ms a step by blocks: 2 sequences of 2,048 tokens 0.519 with
+// 64, 0.526 with 96, 0.655 with 128 and 0.619 on one branch; 4 of 500 0.523, 0.579 (three for a row), 0.661 and 0.615. 71 heads of 64 on one, a block
+// an SM: 8 of 16,384 0.78 with 32, 0.90 with 64 and 0.85 with 24; 16 of 2,048 0.68 with 64, 0.90 with 128.
+int splits_of(long long blocks, int pages, int dp, int nh, bool beside) {
+  const long long slots = beside ? sm_count() / 2 : (nh >= 4 || dp == 256 ? 1ll : 2ll) * sm_count();
   long long want = blocks > 0 ? slots / blocks : 1;
   if (want > pages / 2) want = pages / 2;
+  if (beside && want < MAX_CLUSTER) want = want >= 4 ? 4 : want >= 2 ? 2 : 1;
   if (want > MAX_CLUSTER) {
     const long long wide = (want < pages / 8 ? want : pages / 8) / MAX_CLUSTER * MAX_CLUSTER;
     want = wide > MAX_CLUSTER ? wide : MAX_CLUSTER;
@@ -865,10 +870,15 @@ bool splits_known(int n_splits) { return n_splits >= 1 && n_splits <= 512 && (n_
 
 // Blocks that share a row's pages where the caller leaves it open (n_splits 0). rows: query heads of a K/V head times tokens of a tile, at most;
 // pages: that a row may see, at most. Prompts' last tiles are seldom full: as many chunks of rows are counted as the step's tokens fill.
-static int splits_or(int n_splits, int tiles, int kv_heads, int rows, int tile_tokens, int pages, int tokens, const Plan& q) {
+static int splits_or(int n_splits, int tiles, int kv_heads, int rows, int tile_tokens, int pages, int tokens, const Plan& q, bool beside = false) {
   if (n_splits > 0) return n_splits;
   const long long chunks = ((long long)rows / tile_tokens * tokens + q.rows_pad - 1) / q.rows_pad;
-  return splits_of(kv_heads * (chunks > tiles ? chunks : tiles), pages, q.dp, q.nh);
+  return splits_of(kv_heads * (chunks > tiles ? chunks : tiles), pages, q.dp, q.nh, beside);
+}
+
+// The choice for a step of single tokens that runs beside a weight stream.
+PTB_API int ptb_attention_decode_q8_splits_beside(int seqs, int kv_heads, int rows, int dim, int pages) {
+  return splits_or(0, seqs, kv_heads, rows, 1, pages, seqs, plan_of(dim, rows), true);
 }
 
 // Floats of workspace (`parts` below) of a call that answered PTB_NEEDS_WORKSPACE, for the same sizes; tokens: of the step.

@@ -121,7 +121,8 @@ def lib():
                      "ptb_gla_chunk_tokens", "ptb_delta_prepare", "ptb_delta_walk", "ptb_delta_chunks",
                      "ptb_delta_chunks_supports", "ptb_post_norm", "ptb_token_gate", "ptb_round_rows", "ptb_route_biased", "ptb_attention_tc_sizes", "ptb_attention_tc_supports_sizes", "ptb_attention_tc_extras",
                      "ptb_store_q8", "ptb_unpack_q8", "ptb_copy_pages", "ptb_attention_decode_q8", "ptb_attention_q8",
-                     "ptb_attention_tc_extras_biased", "ptb_pitch_rows"):
+                     "ptb_attention_tc_extras_biased", "ptb_pitch_rows",
+                     "ptb_attention_decode_q8_splits_beside"):
             getattr(L, name).restype = ctypes.c_int
         L.ptb_latent_part_floats.restype = ctypes.c_longlong
         L.ptb_rglru_chunks_work_floats.restype = ctypes.c_longlong
@@ -133,6 +134,7 @@ def lib():
         L.ptb_store_q8.argtypes = [P] * 6 + [I, P, P, P] + [I] * 5 + [P, P]
         L.ptb_unpack_q8.argtypes = [P] * 4 + [I, P, P, P, I, I, P, P, I, I, I, P, P]
         L.ptb_attention_q8_floats.argtypes = [I] * 8
+        L.ptb_attention_decode_q8_splits_beside.argtypes = [I] * 5
         L.ptb_pitch_rows.argtypes = [P, P, N, I, I, P]
         L.ptb_attention_tc_extras_biased.argtypes = [P] * 3 + [I, P, P, P, P, I, P, I, I, I, F, I, P, P]
         L.ptb_attention_decode_q8.argtypes = [P] * 5 + [I, P, P, P, P, I, I, P, I, I, I, F, I, I, I, I, P, N, P, P]
@@ -1964,11 +1966,11 @@ def unpack_pages_q8(k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Ten
 def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.Tensor, v_pool: torch.Tensor, v_exp: torch.Tensor,
                         batch: StepBatchC, rope, slopes: Optional[torch.Tensor], kv_heads: int, q_per_kv: int, head_dim: int,
                         scale: float, window: int = 0, write_cache: bool = True, interleaved: bool = False, n_splits: int = 0,
-                        max_pages: int = 0) -> torch.Tensor:
+                        max_pages: int = 0, beside: bool = False) -> torch.Tensor:
     """The attention of a step of single tokens over a cache in 8 bits: rotate the tokens' queries and keys, append key and value
     to their pages (as ``split_rotate_store_q8`` does), attend. ``n_splits`` blocks share a sequence's pages (more than eight
     in multiples of eight; 0: chosen from the sizes and ``max_pages``, the most pages that a sequence of the step spans, by default the
-    page table's width). At most 128 query heads a K/V head; head sizes are multiples of 16 up to 256. Returns [tokens, heads * head_dim]."""
+    page table's width, and so that room is left for a stream of weights where the call runs ``beside`` one). At most 128 query heads a K/V head; head sizes are multiples of 16 up to 256. Returns [tokens, heads * head_dim]."""
     what = "attention_decode_q8"
     cos, sin, pairs = _check_fused_q8(fused, batch, rope, kv_heads, q_per_kv, head_dim, what)
     device = fused.get_device()
@@ -1985,6 +1987,8 @@ def attention_decode_q8(fused: torch.Tensor, k_pool: torch.Tensor, k_exp: torch.
     if window:
         pages = min(pages, window // PAGE + 2)
     L = lib()
+    if beside and n_splits == 0 and n > 0:
+        n_splits = L.ptb_attention_decode_q8_splits_beside(n, kv_heads, q_per_kv, head_dim, pages)
     out = fused.new_empty((n, heads * head_dim))
     args = (fused.data_ptr(), k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), pool_pages, out.data_ptr(),
             ctypes.byref(batch), cos, sin, pairs, interleaved, slopes_at, heads, kv_heads, head_dim, scale, window, write_cache, n_splits, pages)

@@ -98,8 +98,9 @@ class Attention(Part):
             return False
         lengths = (p + n for p, n in zip(ctx.past, ctx.new))
         keys = sum(min(t, self.window) if self.window else t for t in lengths)
-        size = 2 if getattr(getattr(ctx, "cache", None), "kv_dtype", None) is None else 1
-        return self.build.kernels.decode_attention_fits_beside(keys * self.kv_heads * self.head_dim * 2 * size, self.head_dim)
+        # as many keys in 8 bits as in bfloat16: what they take from the stream is SMs and time more than memory (six layers of 32 heads of 128 on
+        # 8, 4 sequences of 2,048, 34 MB as bfloat16: 0.83 ms a step beside the stream, 0.64 after it)
+        return self.build.kernels.decode_attention_fits_beside(keys * self.kv_heads * self.head_dim * 2 * 2, self.head_dim)
 
     fuses_add = True
 
@@ -160,7 +161,7 @@ class Attention(Part):
         if tokens == 1 and self.q_per_kv <= k.Q8_MAX_HEADS:
             return k.attention_decode_q8(fused, *cache, batch, rope, slopes, self.kv_heads, self.q_per_kv, self.head_dim, self.scale,
                                          window=self.window, write_cache=entry.writes_cache, interleaved=interleaved,
-                                         max_pages=ctx.pages_hint)
+                                         max_pages=ctx.pages_hint, beside=getattr(ctx, "side_stream", None) is not None)
         q = k.split_rotate_store_q8(fused, *cache, batch, self.kv_heads, self.q_per_kv, self.head_dim, write_cache=entry.writes_cache,
                                     rope=rope, interleaved=interleaved)
         first = [max(0, p - self.window + 1) // k.PAGE if self.window > 0 else 0 for p in ctx.past]
