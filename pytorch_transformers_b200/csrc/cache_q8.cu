@@ -218,7 +218,13 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
     auto count = [&](int s) { return sb.seq_new[s] > 0 ? (sb.seq_past[s] + sb.seq_new[s] + PTB_PAGE - 1) / PTB_PAGE - low(s) : 0; };
     if (g == 0 && job + 1 == int(gridDim.x)) {      // 55: the step spans more pages than the workspace has
       int more = job + 1;
-      if (find_job(sb.n_seqs, more, count) >= 0 && tid == 0) atomicExch(p.error_flag, 55);
+      if (find_job(sb.n_seqs, more, count) >= 0) {
+        if (tid == 0) atomicExch(p.error_flag, 55);
+        for (int s = 0, before = 0; s < sb.n_seqs; before += count(s++))      // the places without one name a page that there is
+          for (int i = tid; i < count(s); i += 256)
+            if (before + i > job && (low(s) + i < sb.pages_stride || (i == 0 && sb.pages_stride > 0)))
+              p.table[size_t(s) * sb.pages_stride + min(low(s) + i, sb.pages_stride - 1)] = 0;
+      }
     }
     const int seq = find_job(sb.n_seqs, local, count);
     if (seq < 0) return;
@@ -226,7 +232,11 @@ __global__ void __launch_bounds__(256) unpack_q8_kernel(StepBatch sb, UnpackPara
     const bool listed = index < sb.pages_stride;      // a table too narrow for its sequence is neither read nor written past a row's end
     page = listed ? sb.pages[size_t(seq) * sb.pages_stride + index] : -1;
     valid = min(PTB_PAGE, sb.seq_past[seq] + sb.seq_new[seq] - index * PTB_PAGE);
-    if (listed && g == 0 && tid == 0) p.table[size_t(seq) * sb.pages_stride + index] = job;
+    if (g == 0 && tid == 0) {
+      int* row = p.table + size_t(seq) * sb.pages_stride;
+      if (listed) row[index] = job;
+      else if (local == 0 && sb.pages_stride > 0) row[sb.pages_stride - 1] = job;      // no place of the row is the sequence's: what stands for all
+    }
   }
   const bool known = page >= 0 && page < p.pool_pages;
   if (!known) {

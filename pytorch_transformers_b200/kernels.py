@@ -2074,8 +2074,8 @@ def _attention_q8_unpacked(q, k_pool, k_exp, v_pool, v_exp, batch, tile_seq, til
     n, heads, head_dim = q.shape
     k, v = workspace
     device, wide = q.device, k.shape[-1]
-    # entries that unpacking leaves out (a table too narrow, more pages than n_pages: both are said) name a page that there is
-    table = torch.zeros((batch.n_seqs, max(1, batch.pages_stride)), dtype=torch.int32, device=device)
+    # unpacking fills what the prompt kernel reads of it
+    table = (torch.empty if batch.pages_stride > 0 else torch.zeros)((batch.n_seqs, max(1, batch.pages_stride)), dtype=torch.int32, device=device)
     L, flag, stream = lib(), _flag_at(device.index), _raw_stream(device.index)
     _check(L.ptb_unpack_q8(k_pool.data_ptr(), k_exp.data_ptr(), v_pool.data_ptr(), v_exp.data_ptr(), k_pool.shape[0], None,
                            ctypes.byref(batch), table.data_ptr(), n_pages, window, k.data_ptr(), v.data_ptr(), kv_heads, head_dim,

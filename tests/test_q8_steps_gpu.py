@@ -117,3 +117,21 @@ def test_a_prompt_without_room_for_a_workspace_reads_the_codes(K):
     unpacked = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 8, 0.1, n_pages=pages)
     # each off by its rounding (2^-8) and by weights of 11 bits beside values up to 5.5 (2^-11 of them)
     torch.testing.assert_close(unpacked.float(), want.float(), rtol=2.0 ** -7, atol=2.0 ** -7)
+
+
+@pytest.mark.parametrize("window,width,n_pages", [(0, 2, 3), (70, 1, 1), (64, 2, 2), (500, 9, 4)])
+def test_a_prompt_with_too_few_pages_behind_a_table_too_narrow_is_said(K, window, width, n_pages):
+    c = Case(1, 2, 64, [300, 5, 300], [64, 130, 300], window=window, seed=3)
+    q = c.split()[0].to(BF).cuda()
+    c.append()
+    whole, c.table = c.table, c.table[:, :width].contiguous()
+    cache, batch = c.device(K)
+    lists, n_tiles = tiles_of(c.news, 128)
+    K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 1, c.scale, window=window, n_pages=n_pages)
+    with pytest.raises(K.KernelError, match="page"):
+        K.check_device_errors("cuda")
+    c.table = whole      # and the next step is none the worse
+    cache, batch = c.device(K)
+    out = K.attention_q8(q, *cache, batch, *lists, n_tiles, 128, None, 1, c.scale, window=window, n_pages=24)
+    c.check(out, q.cpu().float())
+    K.check_device_errors("cuda")
