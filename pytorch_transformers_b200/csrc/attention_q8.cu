@@ -36,12 +36,12 @@
 // each warp for itself (a tile's copies a quarter of its time), boxes of 16 or 32 rows asked for by the reading warp or by one warp for
 // all (the requests alone 175 us where memory allows 150).
 //
-// What bounds it: 64 sequences of up to 8,192 keys, 32 heads of 128 on 8, 1 GB of codes: 168 us, 5.8 TB/s; without the arithmetic
-// the same copies take 150, the rate of a plain copy. The ALU pipe is at 46 % of its peak: 181 of 355 instructions for 16 keys, of which
+// What bounds it: 64 sequences of up to 8,192 keys, 32 heads of 128 on 8, 1 GB of codes: 174 us, 5.6 TB/s; without the arithmetic
+// the same copies take 150, the rate of a plain copy. The ALU pipe is at 44 % of its peak: 176 of 361 instructions for 16 keys, of which
 // unpacking and putting pairs together are 80 by the source's count; the rest are maxima, factors and the loop. Few rows and short
 // contexts: the shortest walks measured take 9 us in all, a chain of look-ups (position, page, exponents, codes), queries and the join.
 // 71 heads on one K/V head: 64 sequences of 4,096 keys are slower here than over bfloat16 pages on the tcgen05 kernel (a step of six
-// layers 1.15 against 0.87 ms).
+// layers 1.09 against 0.87 ms).
 #include <cooperative_groups.h>
 
 #include <type_traits>
