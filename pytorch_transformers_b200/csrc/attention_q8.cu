@@ -12,7 +12,8 @@
 // are the unit of the float32 output, which is multiplied by a power of two (exactly) where the unit changes. The unit is
 // a warp's, for all of its rows, and stays within 2^60 of the largest exponent that it has met, so that the output cannot overflow in
 // small units; products with smaller pages are scaled in float32 before they are added. So a row that does not see (or weigh) the large
-// page keeps the small ones' values, to 2^190 below; smaller ones are lost to it. The running maximum moves only when a score exceeds it by 2^4 (one vote a tile instead of shuffles for each row).
+// page keeps the small ones' values: those of pages after it to 2^190 below, those of pages before it to 2^140; smaller ones are lost to
+// it. The running maximum moves only when a score exceeds it by 2^4 (one vote a tile instead of shuffles for each row).
 //
 // A weight's range is float16's: the sum of the weights is float32 and loses none, so a weight too small for float16 would be missing
 // from the output. The largest is therefore at the top, 2^11 to 2^15, and never below 2^5 in a page of values 2^6 below the unit's: 11

@@ -145,3 +145,23 @@ def test_the_smallest_values(K, e, splits):
     want, parts = c.attend(c.split()[0])
     over = (out.cpu().double().view(want.shape) - want).abs() - plain.bound(*parts[0]) - 2.0 ** -134
     assert float(over.max()) <= 0 and bool((out != 0).any())
+
+
+@pytest.mark.parametrize("kv,qpk,dim", [(1, 2, 64), (2, 1, 128), (1, 2, 256), (1, 5, 80)])
+@pytest.mark.parametrize("sizes", [(60, -126, -126), (30, 60, -120, -126, -126)])
+@pytest.mark.parametrize("tile", [64, 128])
+def test_rows_left_of_whose_window_the_largest_values_lie(K, kv, qpk, dim, sizes, tile):
+    # up to 2^186 above; the output's own last place is bfloat16's smallest, 2^-133
+    n = PAGE * len(sizes)
+    c = Case(kv, qpk, dim, [0], [n], window=64, seed=dim)
+    f = c.fused.view(n, kv, qpk + 2, dim)
+    f[:, :, qpk + 1] *= torch.exp2(torch.tensor(sizes).repeat_interleave(PAGE).float())[:, None, None]
+    q = c.split()[0].to(BF)
+    c.append()
+    cache, batch = c.device(K)
+    lists, n_tiles = tiles_of(c.news, tile)
+    out = K.attention_q8(q.cuda(), *cache, batch, *lists, n_tiles, tile, None, kv, c.scale, window=64)
+    want, parts = c.attend(q.float())
+    over = (out.cpu().double().view(want.shape) - want).abs() - plain.bound(*parts[0]) - 2.0 ** -134
+    assert float(over.max()) <= 0
+    K.check_device_errors("cuda")
